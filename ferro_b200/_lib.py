@@ -159,6 +159,21 @@ SIGNATURES = {
                                   c_f32p, C.c_void_p, u64]),
     "fb_mse_fwd_bwd": (C.c_int, [c_stream, c_f32p, c_f32p, u64, f32, c_f32p, c_f32p, C.c_void_p,
                                  u64]),
+    "fb_rope_turns": (C.c_int, [u64, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double, C.c_double, C.c_void_p]),
+    "fb_rope": (C.c_int, [c_stream, C.POINTER(ViewDesc), c_i64p, u64, i64, c_i64p, u64, C.c_int, f32, C.c_int, c_f32p, u64,
+                          C.c_void_p, i64]),
+    "fb_dropout_fwd": (C.c_int, [c_stream, c_f32p, c_f32p, c_f32p, u64, u64, f32, u64, u64, c_i64p, c_f32p]),
+    "fb_dropout_bwd_workspace_bytes": (u64, [u64, u64]),
+    "fb_dropout_bwd": (C.c_int, [c_stream, c_f32p, u64, u64, f32, u64, u64, c_i64p, c_f32p, c_f32p, C.c_void_p, u64]),
+    "fb_dropout_advance": (C.c_int, [c_stream, c_i64p, u64]),
+    "fb_moe_gate_fwd": (C.c_int, [c_stream, c_f32p, u64, u64, u64, C.c_int, c_f32p, c_i64p]),
+    "fb_moe_gate_bwd": (C.c_int, [c_stream, c_f32p, c_f32p, c_f32p, c_i64p, u64, u64, u64, C.c_int, c_f32p]),
+    "fb_moe_sort_workspace_bytes": (u64, [u64, u64]),
+    "fb_moe_sort": (C.c_int, [c_stream, c_i64p, u64, u64, c_i64p, c_i64p, c_i64p, c_i64p, C.c_void_p, u64]),
+    "fb_moe_dispatch_fwd": (C.c_int, [c_stream, c_f32p, c_i64p, u64, u64, u64, c_f32p, u64]),
+    "fb_moe_dispatch_bwd": (C.c_int, [c_stream, c_f32p, c_i64p, u64, u64, u64, u64, c_f32p]),
+    "fb_moe_combine_fwd": (C.c_int, [c_stream, c_f32p, c_f32p, c_i64p, u64, u64, u64, u64, c_f32p]),
+    "fb_moe_combine_bwd": (C.c_int, [c_stream, c_f32p, c_f32p, c_f32p, c_i64p, u64, u64, u64, u64, c_f32p, c_f32p]),
     "fb_host_ln_create": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),
     "fb_host_ln_device_bytes": (u64, [u64, u64, C.c_int]),
     "fb_host_ln_run": (C.c_int, [C.c_void_p, u64, u64, f32] + [C.c_void_p] * 9 + [C.c_void_p, u64]),

@@ -170,6 +170,26 @@ class View:
     offset: int = 0
 
 
+@dataclass(frozen=True)
+class RopePlan:
+    """Frequencies of a rotary embedding on the device (rope_plan), with what else stays the same from call to call."""
+    turns: "DeviceBuffer"  # i64 [rot_dim / 2]: turns a position, as 64-bit fixed-point fractions
+    rot_dim: int
+    layout: int
+    scale: float
+
+
+@dataclass(frozen=True)
+class MoePlan:
+    """Assignments sorted by expert (moe_sort_dev): where every (token, choice) has its row."""
+    place: "DeviceBuffer"    # i64 [tokens * k]: row of an assignment, -1 where it has none
+    order: Optional["DeviceBuffer"]  # i64 [tokens * k]: assignment of a row
+    offsets: "DeviceBuffer"  # i64 [experts + 1]: first row of every expert, then their total
+    tokens: int
+    k: int
+    experts: int
+
+
 class DeviceBuffer:
     """`dyn DeviceBuffer` (dispatch.rs:143-147): whole contiguous device storage."""
 
@@ -223,6 +243,8 @@ class CudaBackend:
         # One non-default stream per backend, like lib.rs:308-312.
         self.stream = torch.cuda.Stream(device=self.device)
         self._ws = None
+        with torch.cuda.stream(self.stream):
+            self._bad_expert = torch.zeros(1, dtype=torch.int64, device=self.device)  # see check_experts
 
     # -- plumbing ---------------------------------------------------------------
     def _s(self):
@@ -866,3 +888,229 @@ class CudaBackend:
         self._check(self.lib.fb_mse_fwd_bwd(self._s(), pred.ptr, target.ptr, len(pred), grad_scale, loss.ptr,
                                             dp.ptr if dp else None, ws, nb))
         return loss, dp
+
+    # -- what a transformer layer runs between its matrix products: shared checks -----------------------
+    def _want(self, what, buf, n, i64=False):
+        """`buf` is n elements of f32 (i64) on this device; None passes."""
+        if buf is None:
+            return None
+        if buf.device != self.device:
+            raise Unsupported("buffer belongs to another device")
+        if buf.is_i64 != i64:
+            raise Unsupported(f"{what} must be an {'i64' if i64 else 'f32'} buffer")
+        if len(buf) != n:
+            raise InvalidShape(f"{what} has {len(buf)} elements, expected {n}")
+        return buf.ptr
+
+    def _scratch(self, nbytes):
+        """Scratch of one call: stream-ordered, and inside a capture owned by the graph's own pool."""
+        if not nbytes:
+            return None
+        with torch.cuda.stream(self.stream):
+            return torch.empty(int(nbytes), dtype=torch.uint8, device=self.device)
+
+    # -- rotary positions ---------------------------------------------------------------------------------
+    ROPE_LAYOUTS = {"interleaved": K.ROPE_INTERLEAVED, "half": K.ROPE_HALF}
+    ROPE_SCALINGS = {"plain": K.ROPE_PLAIN, "linear": K.ROPE_LINEAR, "base": K.ROPE_BASE, "by_parts": K.ROPE_BY_PARTS}
+
+    def rope_plan(self, rot_dim, base=10000.0, layout="half", scaling="plain", factor=1.0, original_len=0.0, low=0.0,
+                  high=0.0, scale=1.0) -> RopePlan:
+        """Frequencies base^(-2i / rot_dim), stretched for long contexts as fb_rope_scaling says; `scale` multiplies cosine
+        and sine.  Built once, kept by the program."""
+        if layout not in self.ROPE_LAYOUTS or scaling not in self.ROPE_SCALINGS:
+            raise InvalidArgument(f"rope_plan: unknown layout {layout!r} or scaling {scaling!r}")
+        if rot_dim < 2 or rot_dim % 2:
+            raise InvalidShape(f"rope_plan: rot_dim {rot_dim} is not an even number from 2 on")
+        turns = np.empty(rot_dim // 2, np.int64)
+        self._check(self.lib.fb_rope_turns(rot_dim, base, self.ROPE_SCALINGS[scaling], factor, original_len, low, high,
+                                           turns.ctypes.data))
+        return RopePlan(self.alloc_i64_from_host(turns), int(rot_dim), self.ROPE_LAYOUTS[layout], float(scale))
+
+    def _rope(self, x, shape, plan, positions, start, inverse, out):
+        if len(shape) != 4:
+            raise InvalidShape(f"rope: shape {list(shape)} is not [batch, seq, heads, head_dim]")
+        b, s, h, d = (int(n) for n in shape)
+        row_major = (s * h * d, h * d, d, 1)
+        if isinstance(x, DeviceBuffer):
+            if len(x) != b * s * h * d:
+                raise InvalidShape(f"rope: {len(x)} elements for shape {list(shape)}")
+            x = View(x, row_major, 0)
+        if out is None:
+            out = self._alloc(b * s * h * d)
+        if isinstance(out, DeviceBuffer):
+            if len(out) != b * s * h * d:
+                raise InvalidShape(f"rope: out has {len(out)} elements for shape {list(shape)}")
+            out = View(out, row_major, 0)
+        if len(x.strides) != 4 or len(out.strides) != 4:
+            raise InvalidShape("rope: views need four strides")
+        self._own(x.buf, out.buf, plan.turns, positions)
+        if x.buf.is_i64 or out.buf.is_i64:
+            raise Unsupported("rope: x and out must be f32 buffers")
+        rows = 1
+        if positions is not None:
+            if not positions.is_i64:
+                raise Unsupported("rope: positions must be an i64 buffer")
+            if len(positions) not in (s, b * s):
+                raise InvalidShape(f"rope: {len(positions)} positions for batch {b} and sequence {s}")
+            rows = 1 if len(positions) == s else b
+        v = _lib.ViewDesc(x.buf.ptr, len(x.buf), int(x.offset), 4, (C.c_uint64 * _lib.MAX_RANK)(b, s, h, d),
+                          (C.c_int64 * _lib.MAX_RANK)(*x.strides))
+        self._check(self.lib.fb_rope(self._s(), C.byref(v), positions.ptr if positions is not None else None, rows,
+                                     int(start), plan.turns.ptr, plan.rot_dim, plan.layout, plan.scale, inverse,
+                                     out.buf.ptr, len(out.buf), (C.c_int64 * 4)(*out.strides), int(out.offset)))
+        return out.buf
+
+    def rope_dev(self, x, shape, plan: RopePlan, positions: Optional[DeviceBuffer] = None, start=0, out=None) -> DeviceBuffer:
+        """Rotary positions on x (a DeviceBuffer, row-major, or a View) of `shape` [batch, seq, heads, head_dim], at
+        `positions` (i64, one per sequence place, or one per batch entry and place) or at start, start + 1, ...  `out` is a
+        DeviceBuffer (row-major) or a View and may be x itself; None allocates."""
+        return self._rope(x, shape, plan, positions, start, 0, out)
+
+    def rope_backward_dev(self, g, shape, plan: RopePlan, positions: Optional[DeviceBuffer] = None, start=0,
+                          out=None) -> DeviceBuffer:
+        """The gradient of rope_dev: g turned back."""
+        return self._rope(g, shape, plan, positions, start, 1, out)
+
+    # -- dropout --------------------------------------------------------------------------------------------
+    @staticmethod
+    def dropout_counters(n):
+        """Counters that a dropout over n elements consumes: add it to the next call's offset."""
+        return (int(n) + 3) // 4
+
+    def dropout_dev(self, x, bias, residual, p, seed, offset, rows, cols, counter: Optional[DeviceBuffer] = None,
+                    out=None) -> DeviceBuffer:
+        """residual + keep * (x + bias) / (1 - p); bias and residual may be None, out may be x or residual.  The mask is a
+        function of (seed, offset + counter[0], element number); `counter` is a one-element i64 buffer."""
+        n = rows * cols
+        px, pb, pr = self._want("dropout: x", x, n), self._want("dropout: bias", bias, cols), self._want("dropout: residual", residual, n)
+        pc = self._want("dropout: counter", counter, 1, i64=True)
+        if out is None:
+            out = self._alloc(n)
+        self._check(self.lib.fb_dropout_fwd(self._s(), px, pb, pr, rows, cols, p, seed, offset, pc,
+                                            self._want("dropout: out", out, n)))
+        return out
+
+    def dropout_backward_dev(self, g, p, seed, offset, rows, cols, counter: Optional[DeviceBuffer] = None, want_dx=True,
+                             want_dbias=False, dx=None, dbias=None):
+        """(dx | None, dbias | None) with the mask of the forward's seed, offset and counter."""
+        n = rows * cols
+        pg, pc = self._want("dropout_backward: g", g, n), self._want("dropout_backward: counter", counter, 1, i64=True)
+        if dx is None and want_dx:
+            dx = self._alloc(n)
+        if dbias is None and want_dbias:
+            dbias = self._alloc(cols)
+        ws = self._scratch(self.lib.fb_dropout_bwd_workspace_bytes(rows, cols) if dbias is not None else 0)
+        self._check(self.lib.fb_dropout_bwd(self._s(), pg, rows, cols, p, seed, offset, pc,
+                                            self._want("dropout_backward: dx", dx, n),
+                                            self._want("dropout_backward: dbias", dbias, cols),
+                                            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0))
+        return dx, dbias
+
+    def dropout_advance_dev(self, counter: DeviceBuffer, n):
+        """counter[0] += n on the device: a captured step draws new masks at every replay."""
+        self._check(self.lib.fb_dropout_advance(self._s(), self._want("dropout_advance: counter", counter, 1, i64=True), n))
+
+    # -- routed experts ---------------------------------------------------------------------------------------
+    def moe_gate_dev(self, logits, tokens, experts, k, renorm=True, weights=None, ids=None):
+        """(weights f32 [tokens, k], ids i64 [tokens, k]): the k largest logits of every row, descending, ties to the lowest
+        index; a logit of -inf is never chosen, places that stay empty get id -1 and weight 0."""
+        pl = self._want("moe_gate: logits", logits, tokens * experts)
+        if weights is None:
+            weights = self._alloc(tokens * k)
+        if ids is None:
+            ids = self._alloc(tokens * k, torch.int64)
+        self._check(self.lib.fb_moe_gate_fwd(self._s(), pl, tokens, experts, k, 1 if renorm else 0,
+                                             self._want("moe_gate: weights", weights, tokens * k),
+                                             self._want("moe_gate: ids", ids, tokens * k, i64=True)))
+        return weights, ids
+
+    def moe_gate_backward_dev(self, dweights, logits, weights, ids, tokens, experts, k, renorm=True, dlogits=None) -> DeviceBuffer:
+        """dlogits [tokens, experts] from the saved weights and ids (logits may be None with renorm)."""
+        pl = self._want("moe_gate_backward: logits", logits, tokens * experts)
+        pd, pw = (self._want("moe_gate_backward: " + n, b, tokens * k) for n, b in (("dweights", dweights), ("weights", weights)))
+        pi = self._want("moe_gate_backward: ids", ids, tokens * k, i64=True)
+        if dlogits is None:
+            dlogits = self._alloc(tokens * experts)
+        self._check(self.lib.fb_moe_gate_bwd(self._s(), pd, pl, pw, pi, tokens, experts, k, 1 if renorm else 0,
+                                             self._want("moe_gate_backward: dlogits", dlogits, tokens * experts)))
+        return dlogits
+
+    def moe_sort_dev(self, ids, tokens, k, experts, place=None, order=None, offsets=None) -> MoePlan:
+        """Assignments sorted by expert, stable.  An id outside [-1, experts) counts as -1 and is reported by
+        check_experts()."""
+        n = tokens * k
+        pi = self._want("moe_sort: ids", ids, n, i64=True)
+        if place is None:
+            place = self._alloc(n, torch.int64)
+        if order is None:
+            order = self._alloc(n, torch.int64)
+        if offsets is None:
+            offsets = self._alloc(experts + 1, torch.int64)
+        ws = self._scratch(self.lib.fb_moe_sort_workspace_bytes(n, experts))
+        self._check(self.lib.fb_moe_sort(self._s(), pi, n, experts, self._want("moe_sort: place", place, n, i64=True),
+                                         self._want("moe_sort: order", order, n, i64=True),
+                                         self._want("moe_sort: offsets", offsets, experts + 1, i64=True), self._bad_expert.data_ptr(),
+                                         ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0))
+        return MoePlan(place, order, offsets, int(tokens), int(k), int(experts))
+
+    def check_experts(self):
+        """Raises if a moe_sort_dev since the last check saw an expert id out of range."""
+        self.synchronize()
+        bad = int(self._bad_expert.item())
+        if bad:
+            with torch.cuda.stream(self.stream):
+                self._bad_expert.zero_()
+            raise InvalidShape(f"moe_sort: expert id at assignment {bad - 1} out of range")
+
+    def _moe_rows(self, what, buf, cols):
+        """Rows of an expert-sorted buffer: as many as it holds."""
+        if cols == 0:
+            return 0
+        if len(buf) % cols:
+            raise InvalidShape(f"{what}: {len(buf)} elements are not rows of {cols}")
+        return len(buf) // cols
+
+    def moe_dispatch_dev(self, x, plan: MoePlan, cols, out=None) -> DeviceBuffer:
+        """xs[place[t, j]] = x[t]; rows of xs behind the last assignment are left as they were."""
+        px = self._want("moe_dispatch: x", x, plan.tokens * cols)
+        if out is None:
+            out = self._alloc(plan.tokens * plan.k * cols)
+        rows = self._moe_rows("moe_dispatch", out, cols)
+        self._check(self.lib.fb_moe_dispatch_fwd(self._s(), px, plan.place.ptr, plan.tokens, plan.k, cols,
+                                                 self._want("moe_dispatch: out", out, rows * cols), rows))
+        return out
+
+    def moe_dispatch_backward_dev(self, g, plan: MoePlan, cols, out=None) -> DeviceBuffer:
+        """dx[t] = sum over j of g[place[t, j]]."""
+        rows = self._moe_rows("moe_dispatch_backward", g, cols)
+        pg = self._want("moe_dispatch_backward: g", g, rows * cols)
+        if out is None:
+            out = self._alloc(plan.tokens * cols)
+        self._check(self.lib.fb_moe_dispatch_bwd(self._s(), pg, plan.place.ptr, plan.tokens, plan.k, cols, rows,
+                                                 self._want("moe_dispatch_backward: out", out, plan.tokens * cols)))
+        return out
+
+    def moe_combine_dev(self, ys, weights, plan: MoePlan, cols, out=None) -> DeviceBuffer:
+        """y[t] = sum over j of weights[t, j] * ys[place[t, j]]."""
+        rows = self._moe_rows("moe_combine", ys, cols)
+        py, pw = self._want("moe_combine: ys", ys, rows * cols), self._want("moe_combine: weights", weights, plan.tokens * plan.k)
+        if out is None:
+            out = self._alloc(plan.tokens * cols)
+        self._check(self.lib.fb_moe_combine_fwd(self._s(), py, pw, plan.place.ptr, plan.tokens, plan.k, cols, rows,
+                                                self._want("moe_combine: out", out, plan.tokens * cols)))
+        return out
+
+    def moe_combine_backward_dev(self, g, ys, weights, plan: MoePlan, cols, want_dys=True, want_dweights=True, dys=None,
+                                 dweights=None):
+        """(dys | None, dweights | None); rows of dys behind the last assignment are left as they were; dys may be ys."""
+        pg, pw = self._want("moe_combine_backward: g", g, plan.tokens * cols), self._want("moe_combine_backward: weights", weights, plan.tokens * plan.k)
+        rows = self._moe_rows("moe_combine_backward", ys, cols)
+        if dys is None and want_dys:
+            dys = self._alloc(rows * cols)
+        if dweights is None and want_dweights:
+            dweights = self._alloc(plan.tokens * plan.k)
+        self._check(self.lib.fb_moe_combine_bwd(self._s(), pg, self._want("moe_combine_backward: ys", ys, rows * cols), pw,
+                                                plan.place.ptr, plan.tokens, plan.k, cols, rows,
+                                                self._want("moe_combine_backward: dys", dys, rows * cols),
+                                                self._want("moe_combine_backward: dweights", dweights, plan.tokens * plan.k)))
+        return dys, dweights

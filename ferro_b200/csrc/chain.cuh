@@ -8,6 +8,7 @@
 //                 is broadcast along the row).
 #pragma once
 #include "common.cuh"
+#include "fastdiv.cuh"
 #include "math.cuh"
 
 namespace fb {
@@ -15,23 +16,6 @@ namespace fb {
 constexpr int kMaxOps = FB_CHAIN_MAX_OPERANDS;
 constexpr int kMaxSteps = FB_CHAIN_MAX_STEPS;
 constexpr int kChThreads = 256;
-
-// n / d for n < 2^31 with one multiply-high (d >= 1).
-struct FastDiv {
-  uint32_t d, magic, shift;
-};
-inline FastDiv make_fastdiv(uint32_t d) {
-  FastDiv f;
-  f.d = d;
-  uint32_t shift = 0;
-  while (shift < 32 && (1ull << shift) < d) ++shift;
-  f.shift = shift;
-  f.magic = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  return f;
-}
-__device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) {
-  return (uint32_t)(((uint64_t)__umulhi(n, f.magic) + n) >> f.shift);
-}
 
 struct Step {
   int8_t opcode, dst, kind, swap;  // kind: public or internal (math.cuh) code

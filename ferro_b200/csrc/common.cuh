@@ -19,6 +19,8 @@ namespace fb {
 // ---- host: errors -------------------------------------------------------
 int fail(int code, const char* fmt, ...);   // sets fb_last_error(), returns code
 int cuda_fail(cudaError_t e, const char* what);
+// Rank, element count, storage pointer and bounds of a view (views.cu); FB_OK for an empty one.
+int check_view(const char* name, const fb_view* v);
 
 #define FB_CUDA(expr)                                      \
   do {                                                     \

@@ -1,0 +1,310 @@
+// Rotary positions: pairs of channels of a [batch, seq, heads, head_dim] view
+// turned by position * theta_i, forward and (with the angle negated) backward.
+//
+// Angle.  theta_i is given in turns as a 64-bit fixed-point fraction, so the
+// fraction of a turn at position p is the low 64 bits of p * turns_i: exact
+// integer arithmetic, no range reduction, the same error (|p| * 2^-65 turns) for
+// the first position and the millionth.  Its top 32 bits become a float in
+// [-1, 1) half turns, off by at most 2^-25, which is what sincospif takes.
+//
+// Roofline: HBM, 8 bytes per element.  A thread owns one group of pairs of one
+// token and walks HPT heads with it, so cosine and sine are paid once per HPT
+// heads; all of a thread's loads are issued before the first product.
+#include <cmath>
+
+#include "common.cuh"
+#include "fastdiv.cuh"
+
+namespace fb {
+
+constexpr int kRopeThreads = 256;
+
+struct RopeArgs {
+  const float* x;
+  float* out;
+  const int64_t* pos;    // NULL: start + s
+  const int64_t* turns;
+  int64_t start;
+  int64_t xs[4], os[4];  // element strides of batch, seq, head, channel
+  uint32_t tokens, seq, heads, half;  // half = rot_dim / 2 pairs
+  uint32_t pair_units, units;  // groups of pairs per head; with the groups of copied channels
+  uint32_t upt;                // threads per token: head chunks * units
+  uint32_t tpb, bpt;           // tokens per CTA; CTAs per token
+  uint32_t pos_batch;          // 1: positions have a row per batch entry
+  uint32_t rot;
+  FastDiv d_upt, d_units, d_seq, d_bpt;
+  uint64_t blocks;
+  float scale, sign;
+};
+
+template <int V>
+struct Vec;
+template <> struct Vec<1> { using T = float; };
+template <> struct Vec<2> { using T = float2; };
+template <> struct Vec<4> { using T = float4; };
+
+template <int VEC>
+__device__ __forceinline__ void rope_load(const float* p, float (&v)[VEC]) {
+  using T = typename Vec<VEC>::T;
+  const T t = __ldcs(reinterpret_cast<const T*>(p));
+  *reinterpret_cast<T*>(v) = t;
+}
+template <int VEC>
+__device__ __forceinline__ void rope_store(float* p, const float (&v)[VEC]) {
+  using T = typename Vec<VEC>::T;
+  __stcs(reinterpret_cast<T*>(p), *reinterpret_cast<const T*>(v));
+}
+
+__device__ __forceinline__ void turn_sincos(uint64_t turns, float scale, float sign, float& s, float& c) {
+  const float h = (float)(int32_t)(turns >> 32) * 4.656612873077393e-10f;  // 2^-31: half turns in [-1, 1]
+  sincospif(h, &s, &c);
+  s *= scale * sign;
+  c *= scale;
+}
+
+// A group of pairs is, in the half layout, VEC neighbours of the first half and the VEC across from
+// them; in the interleaved layout VEC / 2 pairs in one vector (VEC 1: the two channels of one pair,
+// any channel stride).
+template <int VEC, int LAYOUT, int HPT>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs A) {
+  constexpr bool kTwo = LAYOUT == FB_ROPE_HALF || VEC == 1;  // two vectors per group
+  constexpr int kPairs = LAYOUT == FB_ROPE_HALF ? VEC : (VEC + 1) / 2;
+  for (uint64_t blk = blockIdx.x; blk < A.blocks; blk += gridDim.x) {
+    uint32_t token, rem;
+    if (A.bpt == 1) {
+      const uint32_t tl = fdiv(threadIdx.x, A.d_upt);
+      rem = threadIdx.x - tl * A.upt;
+      token = (uint32_t)blk * A.tpb + tl;
+      if (tl >= A.tpb || token >= A.tokens) continue;
+    } else {
+      const uint64_t t = blk / A.bpt;
+      token = (uint32_t)t;
+      rem = (uint32_t)(blk - t * A.bpt) * kRopeThreads + threadIdx.x;
+      if (rem >= A.upt) continue;
+    }
+    const uint32_t chunk = fdiv(rem, A.d_units), u = rem - chunk * A.units;
+    const uint32_t b = fdiv(token, A.d_seq), s = token - b * A.seq;
+    const uint32_t h0 = chunk * HPT, hn = min((uint32_t)HPT, A.heads - h0);
+    const float* xp = A.x + (int64_t)b * A.xs[0] + (int64_t)s * A.xs[1] + (int64_t)h0 * A.xs[2];
+    float* op = A.out + (int64_t)b * A.os[0] + (int64_t)s * A.os[1] + (int64_t)h0 * A.os[2];
+    if (u < A.pair_units) {
+      const uint32_t pair = u * kPairs;
+      const uint32_t ca = LAYOUT == FB_ROPE_HALF ? pair : 2 * pair;             // channel of the first vector
+      const uint32_t cb = LAYOUT == FB_ROPE_HALF ? pair + A.half : 2 * pair + 1;  // and of the second
+      float va[HPT][VEC], vb[HPT][VEC];
+#pragma unroll
+      for (int h = 0; h < HPT; ++h)
+        if (h < (int)hn) {
+          rope_load<VEC>(xp + (int64_t)h * A.xs[2] + (int64_t)ca * A.xs[3], va[h]);
+          if constexpr (kTwo) rope_load<VEC>(xp + (int64_t)h * A.xs[2] + (int64_t)cb * A.xs[3], vb[h]);
+        }
+      const uint64_t p = A.pos ? (uint64_t)__ldg(A.pos + (A.pos_batch ? token : s)) : (uint64_t)A.start + s;
+      float sn[kPairs], cs[kPairs];
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) turn_sincos(p * (uint64_t)__ldg(A.turns + pair + i), A.scale, A.sign, sn[i], cs[i]);
+#pragma unroll
+      for (int h = 0; h < HPT; ++h)
+        if (h < (int)hn) {
+          if constexpr (kTwo) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const float a = va[h][i], c = vb[h][i];
+              va[h][i] = a * cs[i] - c * sn[i];
+              vb[h][i] = c * cs[i] + a * sn[i];
+            }
+            rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)ca * A.os[3], va[h]);
+            rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)cb * A.os[3], vb[h]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+              const float a = va[h][2 * i], c = va[h][2 * i + 1];
+              va[h][2 * i] = a * cs[i] - c * sn[i];
+              va[h][2 * i + 1] = c * cs[i] + a * sn[i];
+            }
+            rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)ca * A.os[3], va[h]);
+          }
+        }
+    } else {
+      const uint32_t c = A.rot + (u - A.pair_units) * VEC;
+      float v[HPT][VEC];
+#pragma unroll
+      for (int h = 0; h < HPT; ++h)
+        if (h < (int)hn) rope_load<VEC>(xp + (int64_t)h * A.xs[2] + (int64_t)c * A.xs[3], v[h]);
+#pragma unroll
+      for (int h = 0; h < HPT; ++h)
+        if (h < (int)hn) rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)c * A.os[3], v[h]);
+    }
+  }
+}
+
+template <int VEC, int LAYOUT>
+static int rope_launch(cudaStream_t stream, RopeArgs& A, bool in_place, uint32_t head_dim) {
+  A.pair_units = LAYOUT == FB_ROPE_HALF ? A.half / VEC : (VEC == 1 ? A.half : A.half / (VEC / 2));
+  A.units = A.pair_units + (in_place ? 0 : (head_dim - A.rot) / VEC);
+  const uint64_t work = (uint64_t)A.tokens * A.units;
+  const bool few = work * ((A.heads + 3) / 4) < (uint64_t)device_info().sm_count * 2048;
+  const uint32_t hpt = few ? 1 : 4;
+  A.upt = (A.heads + hpt - 1) / hpt * A.units;
+  A.tpb = A.upt < kRopeThreads ? kRopeThreads / A.upt : 1;
+  A.bpt = A.upt < kRopeThreads ? 1 : (A.upt + kRopeThreads - 1) / kRopeThreads;
+  A.d_upt = make_fastdiv(A.upt);
+  A.d_units = make_fastdiv(A.units);
+  A.d_seq = make_fastdiv(A.seq);
+  A.blocks = (uint64_t)((A.tokens + A.tpb - 1) / A.tpb) * A.bpt;
+  const unsigned grid = grid_full(A.blocks);
+  if (few) rope_kernel<VEC, LAYOUT, 1><<<grid, kRopeThreads, 0, stream>>>(A);
+  else rope_kernel<VEC, LAYOUT, 4><<<grid, kRopeThreads, 0, stream>>>(A);
+  FB_LAUNCHED("fb_rope");
+  return FB_OK;
+}
+
+template <int LAYOUT>
+static int rope_vec(cudaStream_t stream, RopeArgs& A, bool in_place, uint32_t head_dim, int vec) {
+  if (vec == 4) return rope_launch<4, LAYOUT>(stream, A, in_place, head_dim);
+  if (vec == 2) return rope_launch<2, LAYOUT>(stream, A, in_place, head_dim);
+  return rope_launch<1, LAYOUT>(stream, A, in_place, head_dim);
+}
+
+// Whether two elements of the view may share an address: dims sorted by stride, each must step over
+// everything the smaller ones span.
+static bool may_self_overlap(const uint64_t* shape, const int64_t* strides, int rank) {
+  int idx[FB_MAX_RANK], n = 0;
+  for (int d = 0; d < rank; ++d)
+    if (shape[d] > 1) idx[n++] = d;
+  auto mag = [&](int d) { return strides[d] < 0 ? -(__int128)strides[d] : (__int128)strides[d]; };
+  for (int i = 1; i < n; ++i)
+    for (int j = i; j > 0 && mag(idx[j]) < mag(idx[j - 1]); --j) {
+      const int t = idx[j];
+      idx[j] = idx[j - 1];
+      idx[j - 1] = t;
+    }
+  __int128 span = 0;  // largest offset reached by the dims so far
+  for (int i = 0; i < n; ++i) {
+    if (mag(idx[i]) <= span) return true;
+    span += mag(idx[i]) * (__int128)(shape[idx[i]] - 1);
+  }
+  return false;
+}
+
+// Addresses [lo, hi) that a view touches (bounds already checked, not empty).
+static void touched(const fb_view& v, uintptr_t* lo, uintptr_t* hi) {
+  int64_t a = v.offset, b = v.offset;
+  for (int d = 0; d < v.rank; ++d) {
+    const int64_t span = (int64_t)(v.shape[d] - 1) * v.strides[d];
+    if (span >= 0) b += span;
+    else a += span;
+  }
+  *lo = reinterpret_cast<uintptr_t>(v.ptr + a);
+  *hi = reinterpret_cast<uintptr_t>(v.ptr + b + 1);
+}
+
+}  // namespace fb
+
+using namespace fb;
+
+extern "C" {
+
+int fb_rope_turns(uint64_t rot_dim, double base, int scaling, double factor, double original_len, double low,
+                  double high, int64_t* turns_host) {
+  const char* name = "fb_rope_turns";
+  if (rot_dim < 2 || (rot_dim & 1) || rot_dim > (1u << 30))
+    return fail(FB_ERR_INVALID_SHAPE, "%s: rot_dim %llu is not an even number from 2 on", name, (unsigned long long)rot_dim);
+  if (scaling < FB_ROPE_PLAIN || scaling > FB_ROPE_BY_PARTS) return fail(FB_ERR_INVALID_ARG, "%s: unknown scaling %d", name, scaling);
+  if (!(base > 0.0) || std::isinf(base)) return fail(FB_ERR_INVALID_ARG, "%s: base must be positive and finite", name);
+  if (scaling != FB_ROPE_PLAIN && (!(factor > 0.0) || std::isinf(factor)))
+    return fail(FB_ERR_INVALID_ARG, "%s: factor must be positive and finite", name);
+  if (scaling == FB_ROPE_BASE && rot_dim == 2) return fail(FB_ERR_INVALID_ARG, "%s: one pair has no base to change", name);
+  if (scaling == FB_ROPE_BY_PARTS && (!(original_len > 0.0) || std::isinf(original_len) || !(high > low) || std::isinf(high) || std::isinf(low)))
+    return fail(FB_ERR_INVALID_ARG, "%s: original_len must be positive and low < high", name);
+  if (!turns_host) return fail(FB_ERR_INVALID_ARG, "%s: null table", name);
+  const long double two_pi = 6.283185307179586476925286766559005768L;
+  long double b = base;
+  if (scaling == FB_ROPE_BASE) b *= powl((long double)factor, (long double)rot_dim / (long double)(rot_dim - 2));
+  for (uint64_t i = 0; i < rot_dim / 2; ++i) {
+    long double theta = powl(b, -2.0L * (long double)i / (long double)rot_dim);
+    if (scaling == FB_ROPE_LINEAR) theta /= (long double)factor;
+    if (scaling == FB_ROPE_BY_PARTS) {
+      long double keep = ((long double)original_len * theta / two_pi - low) / ((long double)high - low);
+      keep = keep < 0.0L ? 0.0L : keep > 1.0L ? 1.0L : keep;
+      theta = theta * keep + theta / (long double)factor * (1.0L - keep);
+    }
+    long double t = theta / two_pi;
+    t -= floorl(t);  // whole turns change nothing
+    const long double f = ldexpl(t, 64);  // below 2^64: t < 1
+    uint64_t r = (uint64_t)f;
+    if (f - (long double)r >= 0.5L) ++r;
+    turns_host[i] = (int64_t)r;
+  }
+  return FB_OK;
+}
+
+int fb_rope(fb_stream_t stream, const fb_view* x, const int64_t* positions, uint64_t position_rows, int64_t start,
+            const int64_t* turns, uint64_t rot_dim, int layout, float scale, int inverse, float* out,
+            uint64_t out_len, const int64_t* out_strides, int64_t out_offset) {
+  const char* name = "fb_rope";
+  if (layout != FB_ROPE_INTERLEAVED && layout != FB_ROPE_HALF) return fail(FB_ERR_INVALID_ARG, "%s: unknown layout %d", name, layout);
+  if (int rc = check_view(name, x)) return rc;
+  if (x->rank != 4) return fail(FB_ERR_INVALID_SHAPE, "%s: the view has rank %d, not [batch, seq, heads, head_dim]", name, x->rank);
+  const uint64_t B = x->shape[0], S = x->shape[1], H = x->shape[2], D = x->shape[3];
+  if (rot_dim < 2 || (rot_dim & 1) || rot_dim > D)
+    return fail(FB_ERR_INVALID_SHAPE, "%s: rot_dim %llu is not an even number from 2 to head_dim %llu", name,
+                (unsigned long long)rot_dim, (unsigned long long)D);
+  if (positions && position_rows != 1 && position_rows != B)
+    return fail(FB_ERR_INVALID_SHAPE, "%s: %llu rows of positions for a batch of %llu", name,
+                (unsigned long long)position_rows, (unsigned long long)B);
+  fb_view o = *x;
+  o.ptr = out;
+  o.len = out_len;
+  o.offset = out_offset;
+  int64_t expect = 1;
+  for (int d = 3; d >= 0; --d) {
+    o.strides[d] = out_strides ? out_strides[d] : expect;
+    expect *= (int64_t)x->shape[d];
+  }
+  if (B == 0 || S == 0 || H == 0) return FB_OK;
+  if (int rc = check_view(name, &o)) return rc;
+  if (!turns) return fail(FB_ERR_INVALID_ARG, "%s: null table of frequencies", name);
+  if (B * S >= (1ull << 31) || H * D >= (1ull << 31))
+    return fail(FB_ERR_UNSUPPORTED, "%s: batch * seq or heads * head_dim of 2^31 or more is not supported", name);
+  if (may_self_overlap(o.shape, o.strides, 4)) return fail(FB_ERR_INVALID_ARG, "%s: elements of out share addresses", name);
+  bool in_place = o.ptr + o.offset == x->ptr + x->offset;
+  for (int d = 0; d < 4; ++d) in_place = in_place && (o.shape[d] == 1 || o.strides[d] == x->strides[d]);
+  if (!in_place) {
+    uintptr_t xl, xh, ol, oh;
+    touched(*x, &xl, &xh);
+    touched(o, &ol, &oh);
+    if (xl < oh && ol < xh) return fail(FB_ERR_INVALID_ARG, "%s: out overlaps x without being the same view", name);
+  }
+  RopeArgs A = {};
+  A.x = x->ptr + x->offset;
+  A.out = out + out_offset;
+  A.pos = positions;
+  A.pos_batch = positions && position_rows == B;
+  A.turns = turns;
+  A.start = start;
+  // A vector of `vec` channels needs unit channel strides, addresses that are multiples of its size
+  // and group ends that fall on vector ends.
+  int vec = 4;
+  auto fits = [&](const float* p, const int64_t* st) {
+    for (int d = 0; d < 3; ++d)
+      if (o.shape[d] > 1 && st[d] % vec) return false;
+    return st[3] == 1 && reinterpret_cast<uintptr_t>(p) % (4u * vec) == 0;
+  };
+  while (vec > 1 && !((layout == FB_ROPE_HALF ? rot_dim / 2 : rot_dim) % vec == 0 && D % vec == 0 && fits(A.x, x->strides) && fits(A.out, o.strides)))
+    vec >>= 1;
+  for (int d = 0; d < 4; ++d) {
+    A.xs[d] = o.shape[d] == 1 ? 0 : x->strides[d];
+    A.os[d] = o.shape[d] == 1 ? 0 : o.strides[d];
+  }
+  A.tokens = (uint32_t)(B * S);
+  A.seq = (uint32_t)S;
+  A.heads = (uint32_t)H;
+  A.half = (uint32_t)(rot_dim / 2);
+  A.rot = (uint32_t)rot_dim;
+  A.scale = scale;
+  A.sign = inverse ? -1.0f : 1.0f;
+  return layout == FB_ROPE_HALF ? rope_vec<FB_ROPE_HALF>(stream, A, in_place, (uint32_t)D, vec)
+                                : rope_vec<FB_ROPE_INTERLEAVED>(stream, A, in_place, (uint32_t)D, vec);
+}
+
+}  // extern "C"

@@ -237,7 +237,7 @@ struct ViewPlan {
   int64_t min_kept_stride;
 };
 
-static int check_view(const char* name, const fb_view* v) {
+int check_view(const char* name, const fb_view* v) {
   if (!v) return fail(FB_ERR_INVALID_ARG, "%s: null view", name);
   if (v->rank < 1 || v->rank > FB_MAX_RANK) return fail(FB_ERR_INVALID_SHAPE, "%s: rank %d not in 1..%d", name, v->rank, FB_MAX_RANK);
   uint64_t n = 1;

@@ -504,6 +504,124 @@ FB_API int fb_mse_fwd_bwd(fb_stream_t stream, const float* pred, const float* ta
                           float grad_scale, float* loss, float* dpred, void* workspace,
                           uint64_t workspace_bytes);
 
+/* ---- rotary positions -------------------------------------------------------------------- */
+/* Rotary position embedding.  No counterpart on the reference's device path:
+ * composed there from slices, products with host-made cosine / sine tensors and
+ * concatenations.  Pair i of a head, (a, b), at position p becomes
+ *   a' = scale * (a cos(p theta_i) - b sin(p theta_i))
+ *   b' = scale * (b cos(p theta_i) + a sin(p theta_i)),    i < rot_dim / 2;
+ * channels from rot_dim on are copied.  The angle is exact for any i64 position:
+ * theta_i is held in turns (theta_i / 2 pi) as a 64-bit fixed-point fraction, so
+ * p * theta_i modulo one turn is one wrapping integer product, off by at most
+ * |p| * 2^-65 turns, where an f32 product would lose 2^-24 of the whole angle.
+ *   fb_rope_turns  fills HOST memory with that table, rot_dim / 2 entries
+ *                  (fb_rope_scaling says which theta_i; factor is used by every kind
+ *                  but FB_ROPE_PLAIN, original_len / low / high by FB_ROPE_BY_PARTS);
+ *                  upload it once and keep it.
+ *   fb_rope        x is a view of shape [batch, seq, heads, head_dim], any strides
+ *                  (heads may lie outside seq, or in a packed projection);
+ *                  `out` is addressed by out_strides (NULL: row-major over the
+ *                  shape) and out_offset in a buffer of out_len elements.  It may
+ *                  be x itself (same address and strides: rotation in place,
+ *                  channels from rot_dim on untouched), else the two must not
+ *                  overlap, and no two elements of out may share an address.
+ *                  positions: device i64, row-major [position_rows, seq] with
+ *                  position_rows 1 (shared) or batch; NULL: start + 0 .. seq - 1.
+ *                  turns: the table in DEVICE memory.  inverse != 0 turns by
+ *                  -p theta_i: with the same scale that is the backward.
+ * A batch * seq of 2^31 or more, or heads * head_dim of 2^31 or more, is
+ * FB_ERR_UNSUPPORTED. */
+FB_API int fb_rope_turns(uint64_t rot_dim, double base, int scaling, double factor, double original_len, double low,
+                         double high, int64_t* turns_host);
+FB_API int fb_rope(fb_stream_t stream, const fb_view* x, const int64_t* positions, uint64_t position_rows,
+                   int64_t start, const int64_t* turns, uint64_t rot_dim, int layout, float scale, int inverse,
+                   float* out, uint64_t out_len, const int64_t* out_strides, int64_t out_offset);
+
+/* ---- dropout ------------------------------------------------------------------------------ */
+/* Dropout whose mask is a function of (seed, element number) and is never
+ * stored.  No counterpart on the reference's device path.  Over [rows, cols]:
+ *   out = residual + keep * (x + bias[cols]) / (1 - p)     bias, residual may be NULL
+ * A dropped element is exactly 0 (or exactly the residual) whatever x holds, NaN
+ * and infinities included.  Element e (flat, row-major) is kept when word e % 4 of
+ * Philox4x32-10 (Salmon, Moraes, Dror and Shaw, SC 2011) at counter
+ * offset + counter[0] + e / 4 (64 bits, wrapping, in the low two words) under the
+ * key `seed` (low word first) is at least p * 2^32 rounded to the nearest whole
+ * number; p = 0 keeps everything, p = 1 nothing.  A call consumes
+ * ceil(rows * cols / 4) counters: the next call passes an offset further on by
+ * that much.  counter: device i64, may be NULL (0); a captured step advances it
+ * with fb_dropout_advance (counter[0] += n) so that every replay draws new masks.
+ * out may be x or residual.
+ * Backward: dx = keep * g / (1 - p) with the mask of the same seed, offset and
+ * counter; dbias[c] = sum over rows of dx[:, c] when dbias != NULL.  The gradient
+ * of residual is g.  dx may be g; dx == NULL skips writing it.  Scratch (only for
+ * dbias): fb_dropout_bwd_workspace_bytes(rows, cols). */
+FB_API int fb_dropout_fwd(fb_stream_t stream, const float* x, const float* bias, const float* residual, uint64_t rows,
+                          uint64_t cols, float p, uint64_t seed, uint64_t offset, const int64_t* counter, float* out);
+FB_API uint64_t fb_dropout_bwd_workspace_bytes(uint64_t rows, uint64_t cols);
+FB_API int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t cols, float p, uint64_t seed,
+                          uint64_t offset, const int64_t* counter, float* dx, float* dbias, void* workspace,
+                          uint64_t workspace_bytes);
+FB_API int fb_dropout_advance(fb_stream_t stream, int64_t* counter, uint64_t n);
+
+/* ---- routed experts ------------------------------------------------------------------------ */
+/* The memory-bound half of a layer of routed experts; the experts' matrix
+ * products between dispatch and combine stay with cuBLAS.  No counterpart on the
+ * reference's device path.  An assignment is (token t, choice j), number t * k + j.
+ *
+ * Gate: the k largest logits of each row of [tokens, experts] in descending order
+ * (ties: lowest index first; NaN before everything, as fb_max_dim) with weights
+ *   renorm != 0   softmax over the chosen k
+ *   renorm == 0   the chosen entries of the softmax over all experts.
+ * A logit of -inf is masked: never chosen.  A row with fewer than k others gets
+ * id -1 and weight 0 in what is left of its k places (a padded token is a row of
+ * -inf).  ids are i64 [tokens, k].  1 <= k <= min(experts, FB_MOE_MAX_K),
+ * experts <= FB_MOE_MAX_EXPERTS.
+ * Backward, from the saved weights and ids: dlogits [tokens, experts] in full,
+ *   renorm != 0   w_j (dw_j - sum_i w_i dw_i) at ids j, 0 elsewhere (logits may be NULL)
+ *   renorm == 0   p_e ([e = id j] dw_j - sum_i w_i dw_i), p recomputed from logits;
+ * masked entries get 0, ids outside [0, experts) are skipped. */
+#define FB_MOE_MAX_EXPERTS 1024
+#define FB_MOE_MAX_K 32
+FB_API int fb_moe_gate_fwd(fb_stream_t stream, const float* logits, uint64_t tokens, uint64_t experts, uint64_t k,
+                           int renorm, float* weights, int64_t* ids);
+FB_API int fb_moe_gate_bwd(fb_stream_t stream, const float* dweights, const float* logits, const float* weights,
+                           const int64_t* ids, uint64_t tokens, uint64_t experts, uint64_t k, int renorm,
+                           float* dlogits);
+/* Stable counting sort of n assignments by expert id.  Rows of the sorted order
+ * belong to expert 0, then 1, ...; within an expert they keep the order of the
+ * assignments.
+ *   place   [n]            row of assignment a, -1 where its id is -1
+ *   order   [n], may be NULL   assignment of row r, for r < offsets[experts]; rows
+ *                          behind the last are left as they were
+ *   offsets [experts + 1]  first row of every expert, then their total
+ * An id outside [-1, experts) counts as -1; the highest 1 + position of one is
+ * left in *bad_index (device i64, may be NULL; the caller zeroes it).  n < 2^31.
+ * Deterministic: no order depends on scheduling.
+ * Scratch: fb_moe_sort_workspace_bytes(n, experts) (0: none needed). */
+FB_API uint64_t fb_moe_sort_workspace_bytes(uint64_t n, uint64_t experts);
+FB_API int fb_moe_sort(fb_stream_t stream, const int64_t* ids, uint64_t n, uint64_t experts, int64_t* place,
+                       int64_t* order, int64_t* offsets, int64_t* bad_index, void* workspace,
+                       uint64_t workspace_bytes);
+/* Rows to their experts and back.  xs / ys / dxs / dys are [slots, cols] in the
+ * sorted order, place is fb_moe_sort's; a place outside [0, slots) takes no part.
+ *   dispatch_fwd   xs[place[t, j]] = x[t]; other rows of xs are left as they were
+ *   dispatch_bwd   dx[t] = sum over j of dxs[place[t, j]], j ascending (0 for a token without any)
+ *   combine_fwd    y[t] = sum over j of weights[t, j] * ys[place[t, j]], j ascending
+ *   combine_bwd    dys[place[t, j]] = weights[t, j] * dy[t] (other rows left as they were),
+ *                  dweights[t, j] = dy[t] . ys[place[t, j]] (0 where it takes no part);
+ *                  either may be NULL (ys may be, without dweights); dys may be ys.
+ * 1 <= k <= FB_MOE_MAX_K.  No atomics: a row has one writer and sums have a fixed
+ * order.  Two assignments must not share a place.  Outputs must not alias inputs except as said. */
+FB_API int fb_moe_dispatch_fwd(fb_stream_t stream, const float* x, const int64_t* place, uint64_t tokens, uint64_t k,
+                               uint64_t cols, float* xs, uint64_t slots);
+FB_API int fb_moe_dispatch_bwd(fb_stream_t stream, const float* dxs, const int64_t* place, uint64_t tokens, uint64_t k,
+                               uint64_t cols, uint64_t slots, float* dx);
+FB_API int fb_moe_combine_fwd(fb_stream_t stream, const float* ys, const float* weights, const int64_t* place,
+                              uint64_t tokens, uint64_t k, uint64_t cols, uint64_t slots, float* y);
+FB_API int fb_moe_combine_bwd(fb_stream_t stream, const float* dy, const float* ys, const float* weights,
+                              const int64_t* place, uint64_t tokens, uint64_t k, uint64_t cols, uint64_t slots,
+                              float* dys, float* dweights);
+
 /* ---- host-buffer entry ---------------------------------------------------------------- */
 /* LayerNorm forward + backward for tensors that live in HOST memory: what a
  * ferro user gets from alloc_from_host -> layer_norm_dev -> backward ->

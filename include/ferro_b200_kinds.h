@@ -52,6 +52,21 @@ enum fb_binary_kind {
 
 enum fb_reduce_kind { FB_RED_SUM = 0, FB_RED_MEAN = 1 };
 
+/* Channel pairs of a rotary position (fb_rope). */
+enum fb_rope_layout {
+  FB_ROPE_INTERLEAVED = 0, /* channels (2i, 2i + 1) */
+  FB_ROPE_HALF = 1         /* channels (i, i + rot_dim / 2) */
+};
+/* How fb_rope_turns stretches the frequencies theta_i = base^(-2i / rot_dim) for contexts longer than the
+ * one they were made for. */
+enum fb_rope_scaling {
+  FB_ROPE_PLAIN = 0,   /* theta_i */
+  FB_ROPE_LINEAR = 1,  /* theta_i / factor: positions interpolated */
+  FB_ROPE_BASE = 2,    /* base * factor^(rot_dim / (rot_dim - 2)): the slowest pair is slowed by `factor`, the fastest kept */
+  FB_ROPE_BY_PARTS = 3 /* theta_i where it turns more than `high` times within original_len positions, theta_i / factor
+                          where fewer than `low` times, linear in the number of turns between */
+};
+
 /* Return codes.  Zero is success; everything else leaves every output and
  * in-place operand untouched ("on any Err a kernel must have mutated
  * nothing", dispatch.rs:444-446) and sets the thread-local message read by

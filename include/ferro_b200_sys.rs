@@ -38,6 +38,12 @@ pub const FB_BIN_CLAMP_BWD: c_int = 11;
 pub const FB_BIN_KIND_COUNT: c_int = 12;
 pub const FB_RED_SUM: c_int = 0;
 pub const FB_RED_MEAN: c_int = 1;
+pub const FB_ROPE_INTERLEAVED: c_int = 0;
+pub const FB_ROPE_HALF: c_int = 1;
+pub const FB_ROPE_PLAIN: c_int = 0;
+pub const FB_ROPE_LINEAR: c_int = 1;
+pub const FB_ROPE_BASE: c_int = 2;
+pub const FB_ROPE_BY_PARTS: c_int = 3;
 pub const FB_OK: c_int = 0;
 pub const FB_ERR_INVALID_SHAPE: c_int = 1;
 pub const FB_ERR_INVALID_ARG: c_int = 2;
@@ -51,6 +57,8 @@ pub const FB_VERSION: c_int = 1;
 pub const FB_CHAIN_MAX_STEPS: c_int = 32;
 pub const FB_CHAIN_MAX_OPERANDS: c_int = 6;
 pub const FB_LN_STATIC_SCRATCH_BYTES: c_int = 16777216;
+pub const FB_MOE_MAX_EXPERTS: c_int = 1024;
+pub const FB_MOE_MAX_K: c_int = 32;
 pub const FB_DDP_UNIQUE_ID_BYTES: c_int = 128;
 pub const FB_CH_LOAD: c_int = 0;
 pub const FB_CH_UNARY: c_int = 1;
@@ -214,6 +222,20 @@ extern "C" {
     pub fn fb_bias_act_fwd(stream: Stream, x: *const f32, bias: *const f32, act: c_int, rows: u64, cols: u64, out: *mut f32) -> c_int;
     pub fn fb_bias_act_bwd(stream: Stream, g: *const f32, x: *const f32, bias: *const f32, act: c_int, rows: u64, cols: u64, dx: *mut f32, dbias: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
     pub fn fb_mse_fwd_bwd(stream: Stream, pred: *const f32, target: *const f32, n: u64, grad_scale: f32, loss: *mut f32, dpred: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn fb_rope_turns(rot_dim: u64, base: f64, scaling: c_int, factor: f64, original_len: f64, low: f64, high: f64, turns_host: *mut i64) -> c_int;
+    pub fn fb_rope(stream: Stream, x: *const View, positions: *const i64, position_rows: u64, start: i64, turns: *const i64, rot_dim: u64, layout: c_int, scale: f32, inverse: c_int, out: *mut f32, out_len: u64, out_strides: *const i64, out_offset: i64) -> c_int;
+    pub fn fb_dropout_fwd(stream: Stream, x: *const f32, bias: *const f32, residual: *const f32, rows: u64, cols: u64, p: f32, seed: u64, offset: u64, counter: *const i64, out: *mut f32) -> c_int;
+    pub fn fb_dropout_bwd_workspace_bytes(rows: u64, cols: u64) -> u64;
+    pub fn fb_dropout_bwd(stream: Stream, g: *const f32, rows: u64, cols: u64, p: f32, seed: u64, offset: u64, counter: *const i64, dx: *mut f32, dbias: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn fb_dropout_advance(stream: Stream, counter: *mut i64, n: u64) -> c_int;
+    pub fn fb_moe_gate_fwd(stream: Stream, logits: *const f32, tokens: u64, experts: u64, k: u64, renorm: c_int, weights: *mut f32, ids: *mut i64) -> c_int;
+    pub fn fb_moe_gate_bwd(stream: Stream, dweights: *const f32, logits: *const f32, weights: *const f32, ids: *const i64, tokens: u64, experts: u64, k: u64, renorm: c_int, dlogits: *mut f32) -> c_int;
+    pub fn fb_moe_sort_workspace_bytes(n: u64, experts: u64) -> u64;
+    pub fn fb_moe_sort(stream: Stream, ids: *const i64, n: u64, experts: u64, place: *mut i64, order: *mut i64, offsets: *mut i64, bad_index: *mut i64, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn fb_moe_dispatch_fwd(stream: Stream, x: *const f32, place: *const i64, tokens: u64, k: u64, cols: u64, xs: *mut f32, slots: u64) -> c_int;
+    pub fn fb_moe_dispatch_bwd(stream: Stream, dxs: *const f32, place: *const i64, tokens: u64, k: u64, cols: u64, slots: u64, dx: *mut f32) -> c_int;
+    pub fn fb_moe_combine_fwd(stream: Stream, ys: *const f32, weights: *const f32, place: *const i64, tokens: u64, k: u64, cols: u64, slots: u64, y: *mut f32) -> c_int;
+    pub fn fb_moe_combine_bwd(stream: Stream, dy: *const f32, ys: *const f32, weights: *const f32, place: *const i64, tokens: u64, k: u64, cols: u64, slots: u64, dys: *mut f32, dweights: *mut f32) -> c_int;
     pub fn fb_host_ln_create(chunks: c_int, out: *mut *mut HostLn) -> c_int;
     pub fn fb_host_ln_device_bytes(rows: u64, cols: u64, chunks: c_int) -> u64;
     pub fn fb_host_ln_run(h: *mut HostLn, rows: u64, cols: u64, eps: f32, x: *const f32, g: *const f32, weight: *const f32, bias: *const f32, y: *mut f32, dx: *mut f32, mean: *mut f32, rstd: *mut f32, dweight_dbias: *mut f32, device_staging: *mut c_void, staging_bytes: u64) -> c_int;

@@ -1,0 +1,593 @@
+"""Rotary positions, dropout, the router's gate and the expert sort on the GPU, against the 64-bit references of
+tests/layer_reference.py.  Tolerances count roundings (see there); whole numbers, masks and moved rows are exact."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import layer_reference as ref
+from layer_reference import EPS
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def be():
+    from ferro_b200.backend import CudaBackend
+    return CudaBackend(0)
+
+
+def bk():
+    import ferro_b200.backend as b
+    return b
+
+
+def f32(r, *shape):
+    return r.standard_normal(shape).astype(np.float32)
+
+
+def within(got, want, bound, what=""):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert (np.isnan(got) == np.isnan(want)).all(), what
+    with np.errstate(invalid="ignore"):
+        off = np.where(got == want, 0.0, np.abs(got - want)) - bound
+    off = np.where(np.isnan(want), -1.0, off)
+    assert (off <= 0).all(), (what, float(off.max()), np.unravel_index(off.argmax(), off.shape))
+
+
+def bits(a):
+    return np.ascontiguousarray(a, np.float32).view(np.uint32)
+
+
+# ---- rotary positions ------------------------------------------------------------------------------------------------
+
+ROPE_SHAPES = [  # batch, seq, heads, dim, rot
+    (1, 1, 1, 2, 2), (2, 1, 8, 64, 64), (1, 7, 3, 16, 8), (3, 5, 4, 80, 40), (2, 33, 9, 128, 128), (2, 9, 5, 30, 10), (1, 300, 1, 64, 32),
+    (2, 3, 130, 20, 20), (1, 17, 2, 33, 6), (4, 2, 64, 256, 128), (1, 2, 37, 12, 4), (1, 513, 6, 24, 24), (1, 1, 5, 1030, 1028)]
+
+
+def rope_positions(kind, b, s, r):
+    if kind == "count":
+        return None, 0, np.broadcast_to(np.arange(s), (b, s))
+    if kind == "far":
+        return None, 10 ** 6 + 3, np.broadcast_to(np.arange(s) + 10 ** 6 + 3, (b, s))
+    if kind == "shared":
+        p = r.integers(-50, 1 << 20, s)
+        return p, 0, np.broadcast_to(p, (b, s))
+    p = r.integers(0, 1 << 22, (b, s))
+    return p, 0, p
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shape", ROPE_SHAPES)
+@pytest.mark.parametrize("where", ["count", "far", "shared", "own"])
+def test_rope_forward_and_gradient(be, layout, shape, where):
+    b, s, h, d, rot = shape
+    r = np.random.default_rng(b * 1000 + s * 100 + h * 10 + d)
+    pos, start, full = rope_positions(where, b, s, r)
+    scale = 1.25 if rot % 8 else 1.0
+    plan = be.rope_plan(rot, layout=layout, scale=scale)
+    ang = ref.rope_angles(full, ref.rope_theta(rot))
+    P = None if pos is None else be.alloc_i64_from_host(pos)
+    for inverse, fn in ((False, be.rope_dev), (True, be.rope_backward_dev)):
+        x = f32(r, b, s, h, d)
+        got = be.copy_to_host(fn(be.alloc_from_host(x), (b, s, h, d), plan, positions=P, start=start)).reshape(x.shape)
+        within(got, ref.rope(x, ang, layout, scale, inverse), ref.rope_bound(x, rot, layout, scale), (inverse,))
+        assert (bits(got[..., rot:]) == bits(x[..., rot:])).all()  # channels behind the turned ones are copies
+
+
+@pytest.mark.parametrize("scaling,kw", [("linear", dict(factor=4.0)), ("base", dict(factor=8.0)),
+                                        ("by_parts", dict(factor=8.0, original_len=4096.0, low=1.0, high=32.0))])
+def test_rope_scaled_for_long_contexts(be, scaling, kw):
+    b, s, h, d, rot = 1, 50, 2, 64, 48
+    r = np.random.default_rng(7)
+    x = f32(r, b, s, h, d)
+    plan = be.rope_plan(rot, base=500000.0, layout="half", scaling=scaling, scale=1.2, **kw)
+    ang = ref.rope_angles(np.arange(s)[None] + 131072, ref.rope_theta(rot, 500000.0, scaling, **kw))
+    got = be.copy_to_host(be.rope_dev(be.alloc_from_host(x), x.shape, plan, start=131072)).reshape(x.shape)
+    within(got, ref.rope(x, ang, "half", 1.2), ref.rope_bound(x, rot, "half", 1.2))
+
+
+@pytest.mark.parametrize("start", [-1, 2 ** 31 - 2, 2 ** 40])
+def test_rope_positions_beyond_32_bits_and_below_zero(be, start):
+    """The angle is a wrapping integer product: position p turns as exactly as position 0.  The reference multiplies the
+    table's own fractions (whole numbers) so that its own rounding does not enter."""
+    rot, s = 32, 5
+    x = f32(np.random.default_rng(8), 1, s, 1, rot)
+    plan = be.rope_plan(rot)
+    turns = [int(v) % 2 ** 64 for v in be.copy_i64_to_host(plan.turns)]
+    ang = np.array([[[((start + p) * t % 2 ** 64) / 2 ** 64 * 2 * math.pi for t in turns] for p in range(s)]])
+    got = be.copy_to_host(be.rope_dev(be.alloc_from_host(x), x.shape, plan, start=start)).reshape(x.shape)
+    within(got, ref.rope(x, ang, "half"), ref.rope_bound(x, rot, "half"))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shift", [0, 1, 2])
+def test_rope_on_strided_views_in_place_and_into_a_cache(be, layout, shift):
+    """Query heads of a packed projection, heads outside the sequence, addresses that fit no vector, output in place and
+    into a longer buffer: nothing outside the view is touched."""
+    b, s, h, d, rot = 2, 6, 3, 16, 8
+    View = bk().View
+    r = np.random.default_rng(9)
+    plan = be.rope_plan(rot, layout=layout)
+    ang = ref.rope_angles(np.broadcast_to(np.arange(s) + 11, (b, s)), ref.rope_theta(rot))
+    packed = f32(r, b * s * (h + 2) * d + 8)
+    strides, off = (s * (h + 2) * d, (h + 2) * d, d, 1), d + shift
+    x = np.lib.stride_tricks.as_strided(packed[off:], (b, s, h, d), [4 * n for n in strides]).copy()
+    want, bound = ref.rope(x, ang, layout), ref.rope_bound(x, rot, layout)
+    # into heads-outside memory of a longer cache
+    buf = be.alloc_from_host(packed)
+    cache = be.alloc_from_host(np.full(b * h * 10 * d + 4, 7.0, np.float32))
+    out_strides, out_off = (h * 10 * d, d, 10 * d, 1), 2 * d + shift
+    be.rope_dev(View(buf, strides, off), (b, s, h, d), plan, start=11, out=View(cache, out_strides, out_off))
+    got = be.copy_to_host(cache).copy()
+    seen = np.lib.stride_tricks.as_strided(got[out_off:], (b, s, h, d), [4 * n for n in out_strides])
+    within(seen, want, bound)
+    seen[...] = 7.0
+    assert (got == 7.0).all()
+    # in place
+    be.rope_dev(View(buf, strides, off), (b, s, h, d), plan, start=11, out=View(buf, strides, off))
+    got = be.copy_to_host(buf).copy()
+    seen = np.lib.stride_tricks.as_strided(got[off:], (b, s, h, d), [4 * n for n in strides])
+    within(seen, want, bound)
+    seen[...] = np.lib.stride_tricks.as_strided(packed[off:], (b, s, h, d), [4 * n for n in strides])
+    assert (bits(got) == bits(packed)).all()
+    # channels that are not neighbours: a transposed view, and a broadcast batch
+    xt = f32(r, s, h, d, b)
+    tv = View(be.alloc_from_host(xt), (1, h * d * b, d * b, b), 0)
+    xl = xt.transpose(3, 0, 1, 2)
+    got = be.copy_to_host(be.rope_dev(tv, (b, s, h, d), plan, start=11)).reshape(b, s, h, d)
+    within(got, ref.rope(xl, ang, layout), ref.rope_bound(xl, rot, layout))
+    one = f32(r, 1, s, h, d)
+    bv = View(be.alloc_from_host(one), (0, h * d, d, 1), 0)
+    got = be.copy_to_host(be.rope_dev(bv, (b, s, h, d), plan, start=11)).reshape(b, s, h, d)
+    within(got, ref.rope(np.broadcast_to(one, (b, s, h, d)), ang, layout), ref.rope_bound(np.broadcast_to(one, (b, s, h, d)), rot, layout))
+
+
+def test_rope_refusals_of_the_mirror(be):
+    b = bk()
+    x, plan = be.alloc_from_host(np.zeros(64, np.float32)), be.rope_plan(8)
+    with pytest.raises(b.InvalidShape):
+        be.rope_dev(x, (1, 2, 4, 4), plan)            # other number of elements
+    with pytest.raises(b.InvalidShape):
+        be.rope_dev(x, (2, 8, 4), plan)               # no sequence
+    with pytest.raises(b.InvalidShape):
+        be.rope_dev(x, (1, 2, 8, 4), plan)            # rot_dim 8 of 4 channels
+    with pytest.raises(b.InvalidShape):
+        be.rope_dev(x, (2, 2, 2, 8), plan, positions=be.alloc_i64_from_host([1, 2, 3]))
+    with pytest.raises(b.Unsupported):
+        be.rope_dev(x, (2, 2, 2, 8), plan, positions=be.alloc_from_host([1, 2]))
+    with pytest.raises(b.InvalidArgument):
+        be.rope_plan(8, layout="quarter")
+    with pytest.raises(b.InvalidShape):
+        be.rope_plan(7)
+
+
+# ---- dropout ---------------------------------------------------------------------------------------------------------
+
+DROP_SHAPES = [(1, 1), (1, 3), (3, 5), (2, 4), (64, 256), (17, 1001), (5, 4100), (1000, 7), (333, 64), (4099, 33), (1, 100003)]
+
+
+@pytest.mark.parametrize("rows,cols", DROP_SHAPES)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("residual", [False, True])
+def test_dropout_forward_and_gradient(be, rows, cols, bias, residual):
+    r = np.random.default_rng(rows * 7 + cols)
+    p, seed, offset = 0.25 + 0.1 * residual, 0xFEDCBA9876543210 - rows, 2 ** 32 - 5 + cols
+    x, b, res, g = f32(r, rows, cols), f32(r, cols) if bias else None, f32(r, rows, cols) if residual else None, f32(r, rows, cols)
+    dev = lambda a: None if a is None else be.alloc_from_host(a)
+    X, R, G = dev(x), dev(res), dev(g)
+    want, keep, bound = ref.dropout(x, b, res, p, seed, offset)
+    got = be.copy_to_host(be.dropout_dev(X, dev(b), R, p, seed, offset, rows, cols)).reshape(rows, cols)
+    within(got, want, bound)
+    # a dropped element is exactly 0, or exactly the residual
+    assert (bits(got[~keep]) == bits((res if residual else np.zeros_like(x))[~keep])).all()
+    wdx, _, wb = ref.dropout(g, None, None, p, seed, offset)
+    dx, db = be.dropout_backward_dev(G, p, seed, offset, rows, cols, want_dbias=bias)
+    gdx = be.copy_to_host(dx).reshape(rows, cols)
+    within(gdx, wdx, wb)
+    assert ((gdx == 0) == (~keep | (g == 0))).all()  # the same mask again
+    if bias:
+        # at most `rows` additions in a column, each of partial sums below the sum of magnitudes
+        within(be.copy_to_host(db), wdx.sum(0), (rows + 3) * EPS * np.abs(wdx).sum(0) * 1.001)
+        none, only = be.dropout_backward_dev(G, p, seed, offset, rows, cols, want_dx=False, want_dbias=True)
+        assert none is None and (bits(be.copy_to_host(only)) == bits(be.copy_to_host(db))).all()
+    # in place
+    be.dropout_dev(X, dev(b), R, p, seed, offset, rows, cols, out=X)
+    assert (bits(be.copy_to_host(X).reshape(rows, cols)) == bits(got)).all()
+    if residual:
+        be.dropout_dev(dev(x), dev(b), R, p, seed, offset, rows, cols, out=R)
+        assert (bits(be.copy_to_host(R).reshape(rows, cols)) == bits(got)).all()
+    be.dropout_backward_dev(G, p, seed, offset, rows, cols, dx=G)
+    assert (bits(be.copy_to_host(G).reshape(rows, cols)) == bits(gdx)).all()
+
+
+@pytest.mark.parametrize("n,shift", [(1000, 1), (4097, 2), (64, 3), (5, 1)])
+def test_dropout_at_addresses_that_fit_no_vector(be, n, shift):
+    """The mask goes by element number, not by address."""
+    DeviceBuffer = bk().DeviceBuffer
+    r = np.random.default_rng(n)
+    x, b, res = f32(r, n), f32(r, n), f32(r, n)
+    hold = [be.alloc_from_host(np.concatenate([np.zeros(shift, np.float32), a])) for a in (x, b, res, x)]
+    X, B, R, O = (DeviceBuffer(h.t[shift:]) for h in hold)
+    want, keep, bound = ref.dropout(x[None], b, res[None], 0.5, 99, 7)
+    be.dropout_dev(X, B, R, 0.5, 99, 7, 1, n, out=O)
+    within(be.copy_to_host(O)[None], want, bound)
+    aligned = be.dropout_dev(be.alloc_from_host(x), be.alloc_from_host(b), be.alloc_from_host(res), 0.5, 99, 7, 1, n)
+    assert (bits(be.copy_to_host(O)) == bits(be.copy_to_host(aligned))).all()
+    dx, db = be.dropout_backward_dev(X, 0.5, 99, 7, 1, n, want_dbias=True)
+    wdx, _, wb = ref.dropout(x[None], None, None, 0.5, 99, 7)
+    within(be.copy_to_host(dx)[None], wdx, wb)
+    within(be.copy_to_host(db), wdx[0], wb[0])
+
+
+def test_dropout_edges(be):
+    """p of 0 and 1, NaN and infinities in dropped places, counters that wrap, the device-side counter."""
+    r = np.random.default_rng(3)
+    x = f32(r, 8, 36)
+    X = be.alloc_from_host(x)
+    assert (bits(be.copy_to_host(be.dropout_dev(X, None, None, 0.0, 1, 0, 8, 36))) == bits(x.ravel())).all()
+    gone = be.copy_to_host(be.dropout_dev(be.alloc_from_host(x * np.float32(np.inf)), None, X, 1.0, 1, 0, 8, 36))
+    assert (bits(gone) == bits(x.ravel())).all()
+    keep = ref.drop_keep(288, 0.5, 5, 2 ** 64 - 3).reshape(8, 36)
+    y = np.where(keep, x, np.where(r.random((8, 36)) < 0.5, np.nan, np.inf)).astype(np.float32)
+    got = be.copy_to_host(be.dropout_dev(be.alloc_from_host(y), None, None, 0.5, 5, 2 ** 64 - 3, 8, 36)).reshape(8, 36)
+    assert (bits(got) == bits(np.where(keep, 2 * x, 0))).all()  # 1 / (1 - 0.5) is a power of two: exact
+    # offset + counter[0], and the counter's advance
+    c = be.alloc_i64_from_host([100])
+    a = be.copy_to_host(be.dropout_dev(X, None, None, 0.5, 5, 23, 8, 36, counter=c))
+    assert (bits(a) == bits(be.copy_to_host(be.dropout_dev(X, None, None, 0.5, 5, 123, 8, 36)))).all()
+    be.dropout_advance_dev(c, be.dropout_counters(8 * 36))
+    assert be.copy_i64_to_host(c).tolist() == [172]
+    d1, b1 = be.dropout_backward_dev(X, 0.5, 5, 23, 8, 36, counter=c, want_dbias=True)
+    d2, b2 = be.dropout_backward_dev(X, 0.5, 5, 195, 8, 36, want_dbias=True)
+    assert (bits(be.copy_to_host(d1)) == bits(be.copy_to_host(d2))).all() and (bits(be.copy_to_host(b1)) == bits(be.copy_to_host(b2))).all()
+    # empty problems
+    e = be.alloc_from_host(np.zeros(0, np.float32))
+    assert len(be.dropout_dev(e, None, None, 0.5, 5, 0, 0, 36)) == 0
+    _, db = be.dropout_backward_dev(e, 0.5, 5, 0, 0, 36, want_dbias=True)
+    assert be.copy_to_host(db).tolist() == [0.0] * 36
+    b = bk()
+    with pytest.raises(b.InvalidShape):
+        be.dropout_dev(X, be.alloc_from_host(np.zeros(35, np.float32)), None, 0.5, 5, 0, 8, 36)
+    with pytest.raises(b.Unsupported):
+        be.dropout_dev(X, None, None, 0.5, 5, 0, 8, 36, counter=be.alloc_from_host([0.0]))
+    with pytest.raises(b.InvalidArgument):
+        be.dropout_dev(X, None, None, 1.5, 5, 0, 8, 36)
+
+
+# ---- gate --------------------------------------------------------------------------------------------------------------
+
+GATE_SHAPES = [(1, 1, 1), (5, 2, 2), (9, 3, 1), (33, 8, 2), (100, 16, 4), (64, 31, 5), (257, 32, 8), (64, 33, 32), (50, 60, 6), (129, 64, 8),
+               (40, 100, 10), (77, 128, 8), (20, 200, 3), (33, 256, 9), (10, 500, 17), (6, 1000, 32), (5, 1024, 8)]
+
+
+def gate_logits(kind, t, e, r):
+    l = (2 * r.standard_normal((t, e))).astype(np.float32)
+    if kind == "ties":
+        l = np.round(l).astype(np.float32)
+        l[::3] *= 0.0  # +0 and -0: equal
+        l[1::5] = 1.0
+    if kind == "masked":
+        l[r.random((t, e)) < 0.4] = -np.inf
+        l[::4] = -np.inf           # tokens that choose nobody
+        l[1::6, 1:] = -np.inf      # one expert left
+        l[2::6] = np.finfo(np.float32).min  # the lowest finite value is no mask
+    if kind == "wide":
+        l *= np.float32(60)        # exponentials that vanish
+    return l
+
+
+@pytest.mark.parametrize("t,e,k", GATE_SHAPES)
+@pytest.mark.parametrize("kind", ["plain", "ties", "masked", "wide"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_gate_choice_weights_and_gradient(be, t, e, k, kind, renorm):
+    r = np.random.default_rng(t + 31 * e + k)
+    l, dw = gate_logits(kind, t, e, r), f32(r, t, k)
+    L = be.alloc_from_host(l)
+    W, I = be.moe_gate_dev(L, t, e, k, renorm)
+    ww, wi = ref.gate(l, k, renorm)
+    ids, w = be.copy_i64_to_host(I).reshape(t, k), be.copy_to_host(W).reshape(t, k)
+    assert (ids == wi).all()
+    rel = ref.gate_rel(l, k, renorm)
+    within(w, ww, rel * ww + 2.0 ** -125)  # below 2^-126 the f32 exponential has fewer bits
+    assert (w[wi < 0] == 0).all()
+    got = be.copy_to_host(be.moe_gate_backward_dev(be.alloc_from_host(dw), L, W, I, t, e, k, renorm)).reshape(t, e)
+    want = ref.gate_backward(dw, l, wi, k, renorm)
+    # p (dw - dot): p off by rel, dot by rel and its k products and additions, three more roundings
+    mag = np.abs(ww * dw).sum(1, keepdims=True)
+    p = np.abs(ref.gate(l, e, False)[0]).max(1, keepdims=True) if not renorm else ww.max(1, keepdims=True)
+    up = np.abs(dw).max(1, keepdims=True)
+    within(got, want, p * (up + mag) * (2 * rel + (k + 8) * EPS) + 2.0 ** -120)
+    assert (got[l == -np.inf] == 0).all()
+    if renorm:
+        again = be.moe_gate_backward_dev(be.alloc_from_host(dw), None, W, I, t, e, k, True)  # needs no logits
+        assert (bits(be.copy_to_host(again)) == bits(got.ravel())).all()
+
+
+def test_gate_nan_and_infinity(be):
+    l = np.array([[1, np.nan, 3, np.nan], [np.inf, 2, np.inf, 1], [-np.inf, np.inf, 0, -np.inf], [0, -0.0, 0, -0.0]], np.float32)
+    for renorm in (True, False):
+        W, I = be.moe_gate_dev(be.alloc_from_host(l), 4, 4, 3, renorm)
+        assert be.copy_i64_to_host(I).reshape(4, 3).tolist() == [[1, 3, 2], [0, 2, 1], [1, 2, -1], [0, 1, 2]]
+        w = be.copy_to_host(W).reshape(4, 3)
+        assert np.isnan(w[0]).all()                        # a NaN logit: no softmax
+        assert np.isnan(w[1, :2]).all()                    # inf - inf, as in fb_softmax_fwd
+        assert w[2, 2] == 0
+        within(w[3], np.full(3, 1 / 3 if renorm else 1 / 4), 1e-6)
+        # ids outside [0, experts) take no part in the gradient
+        d = be.moe_gate_backward_dev(be.alloc_from_host(np.ones(3, np.float32)), be.alloc_from_host(l[3]), be.alloc_from_host(np.float32([0.5, 0.3, 0.2])),
+                                     be.alloc_i64_from_host([-1, 4, 1 << 40]), 1, 4, 3, renorm)
+        assert (be.copy_to_host(d) == 0).all()
+
+
+# ---- expert sort ---------------------------------------------------------------------------------------------------------
+
+def sort_ids(kind, n, e, r):
+    if kind == "one":
+        return np.full(n, e - 1, np.int64)
+    if kind == "none":
+        return np.full(n, -1, np.int64)
+    if kind == "skewed":
+        return np.minimum((r.exponential(0.15, n) * e).astype(np.int64), e - 1)
+    return r.integers(-1 if kind == "padded" else 0, e, n)
+
+
+@pytest.mark.parametrize("n", [0, 1, 2, 31, 32, 33, 127, 1000, 4095, 4096, 4097, 8192, 20000, 262144, 262145, 300001])
+@pytest.mark.parametrize("e", [1, 7, 64, 1000, 1024])
+@pytest.mark.parametrize("kind", ["even", "skewed", "padded", "one", "none"])
+def test_sort_is_the_stable_counting_sort(be, n, e, kind):
+    ids = sort_ids(kind, n, e, np.random.default_rng(n + e))
+    order = be.alloc_i64_from_host(np.full(n, -77))
+    plan = be.moe_sort_dev(be.alloc_i64_from_host(ids), n, 1, e, order=order)
+    place, want, off = ref.sort_by_expert(ids, e)
+    assert (be.copy_i64_to_host(plan.place) == place).all()
+    got = be.copy_i64_to_host(plan.order)
+    assert (got[:len(want)] == want).all()
+    assert (got[len(want):] == -77).all()  # rows behind the last are left as they were
+    assert (be.copy_i64_to_host(plan.offsets) == off).all()
+    be.check_experts()
+
+
+def test_sort_reports_ids_out_of_range_and_treats_them_as_none(be):
+    for n in (5, 5000, 300000):
+        ids = np.random.default_rng(n).integers(0, 6, n)
+        ids[[1, n - 2]] = [6, -2]
+        ids[3] = 1 << 40
+        plan = be.moe_sort_dev(be.alloc_i64_from_host(ids), n, 1, 6)
+        assert (be.copy_i64_to_host(plan.place) == ref.sort_by_expert(ids, 6)[0]).all()
+        with pytest.raises(bk().InvalidShape, match=f"assignment {n - 2} "):
+            be.check_experts()
+        be.check_experts()  # said once
+
+
+# ---- rows to their experts and back ----------------------------------------------------------------------------------------
+
+ROW_SHAPES = [(1, 1, 1, 1), (5, 2, 3, 4), (7, 3, 3, 130), (3, 4, 2, 1030), (33, 8, 8, 64), (64, 16, 4, 100), (20, 64, 32, 36), (9, 5, 2, 4096), (2, 4, 3, 8200),
+              (130, 12, 6, 31), (12, 9, 9, 257), (4, 40, 17, 516)]
+
+
+@pytest.mark.parametrize("t,e,k,c", ROW_SHAPES)
+@pytest.mark.parametrize("kind", ["even", "padded", "none"])
+def test_rows_to_their_experts_and_back_with_gradients(be, t, e, k, c, kind):
+    r = np.random.default_rng(t + e + k + c)
+    ids = sort_ids(kind, t * k, e, r)
+    x, w, dy = f32(r, t, c), f32(r, t, k), f32(r, t, c)
+    ys, dxs = f32(r, t * k, c), f32(r, t * k, c)
+    plan = be.moe_sort_dev(be.alloc_i64_from_host(ids), t, k, e)
+    place, _, off = ref.sort_by_expert(ids, e)
+    rows = int(off[-1])
+    W, wf = be.alloc_from_host(w), w.ravel()
+    fill = lambda: be.alloc_from_host(np.full((t * k, c), 9.0, np.float32))
+    xs = be.copy_to_host(be.moe_dispatch_dev(be.alloc_from_host(x), plan, c, out=fill())).reshape(t * k, c)
+    assert (bits(xs) == bits(ref.spread(x, place, k, t * k, 9.0))).all()
+    dx = be.copy_to_host(be.moe_dispatch_backward_dev(be.alloc_from_host(dxs), plan, c)).reshape(t, c)
+    want, mag = ref.collect(dxs, place, t, k)
+    within(dx, want, k * EPS * mag)
+    YS = be.alloc_from_host(ys)
+    y = be.copy_to_host(be.moe_combine_dev(YS, W, plan, c)).reshape(t, c)
+    want, mag = ref.collect(ys, place, t, k, wf)
+    within(y, want, (k + 1) * EPS * mag)
+    dys, dw = be.moe_combine_backward_dev(be.alloc_from_host(dy), YS, W, plan, c, dys=fill())
+    gdys, gdw = be.copy_to_host(dys).reshape(t * k, c), be.copy_to_host(dw)
+    wdys = ref.spread(dy, place, k, t * k, 9.0, wf)
+    within(gdys, wdys, EPS * np.abs(wdys))
+    assert (gdys[rows:] == 9.0).all()
+    want, mag = ref.weight_gradient(dy, ys, place, k)
+    within(gdw, want, (math.ceil(c / 32) + 8) * EPS * mag)  # at least 32 threads share a row
+    # one at a time, and the gradient of the rows written over them
+    assert (bits(be.copy_to_host(be.moe_combine_backward_dev(be.alloc_from_host(dy), YS, W, plan, c, want_dys=False)[1])) == bits(gdw)).all()
+    only = be.moe_combine_backward_dev(be.alloc_from_host(dy), YS, W, plan, c, want_dweights=False, dys=fill())
+    assert only[1] is None and (bits(be.copy_to_host(only[0])) == bits(gdys.ravel())).all()
+    over, dw2 = be.moe_combine_backward_dev(be.alloc_from_host(dy), YS, W, plan, c, dys=YS)
+    assert (bits(be.copy_to_host(dw2)) == bits(gdw)).all()
+    assert (bits(be.copy_to_host(over).reshape(t * k, c)[:rows]) == bits(gdys[:rows])).all()
+    assert (bits(be.copy_to_host(over).reshape(t * k, c)[rows:]) == bits(ys[rows:])).all()
+
+
+def test_rows_with_fewer_slots_than_places_and_foreign_addresses(be):
+    """A place outside the buffer's rows takes no part; addresses that fit no vector give the same values."""
+    t, e, k, c = 13, 4, 3, 64
+    r = np.random.default_rng(5)
+    ids = r.integers(0, e, t * k)
+    plan = be.moe_sort_dev(be.alloc_i64_from_host(ids), t, k, e)
+    place = ref.sort_by_expert(ids, e)[0]
+    x, w, ys, dy = f32(r, t, c), f32(r, t, k), f32(r, 20, c), f32(r, t, c)
+    DB = bk().DeviceBuffer
+    for shift in (0, 1):
+        at = lambda a: DB(be.alloc_from_host(np.concatenate([np.zeros(shift, np.float32), np.ravel(a)])).t[shift:])
+        out = at(np.full((20, c), 9.0))
+        got = be.copy_to_host(be.moe_dispatch_dev(at(x), plan, c, out=out)).reshape(20, c)
+        assert (bits(got) == bits(ref.spread(x, place, k, 20, 9.0))).all()
+        want, mag = ref.collect(ys, place, t, k, w.ravel())
+        within(be.copy_to_host(be.moe_combine_dev(at(ys), at(w), plan, c)).reshape(t, c), want, (k + 1) * EPS * mag)
+        dys, dw = be.moe_combine_backward_dev(at(dy), at(ys), at(w), plan, c, dys=at(np.full((20, c), 9.0)))
+        wdys = ref.spread(dy, place, k, 20, 9.0, w.ravel())
+        within(be.copy_to_host(dys).reshape(20, c), wdys, EPS * np.abs(wdys))
+        want, mag = ref.weight_gradient(dy, ys, place, k)
+        within(be.copy_to_host(dw), want, (math.ceil(c / 32) + 8) * EPS * mag)
+    b = bk()
+    with pytest.raises(b.InvalidShape):
+        be.moe_dispatch_dev(be.alloc_from_host(x), plan, c, out=be.alloc_from_host(np.zeros(100, np.float32)))
+    with pytest.raises(b.InvalidShape):
+        be.moe_dispatch_dev(be.alloc_from_host(ys), plan, c)
+    with pytest.raises(b.Unsupported):
+        be.moe_sort_dev(be.alloc_from_host(np.zeros(8, np.float32)), 8, 1, 4)
+
+
+# ---- the layer's run -------------------------------------------------------------------------------------------------------
+
+def test_a_layer_with_routed_experts_forward_and_backward(be):
+    """Rotary positions, then dropout with bias and residual, RMS norm, gate, sort, dispatch, the experts' activation
+    (bias_act_dev stands for their products), combine, dropout with residual: values and every gradient against the same
+    run in 64 bits with torch's own differentiation of the formulas."""
+    b, s, h, d = 2, 9, 3, 16
+    t, c, e, k = b * s, h * d, 6, 2
+    r = np.random.default_rng(21)
+    x, bias, res, wn, wg, up = f32(r, t, c), f32(r, c), f32(r, t, c), f32(r, c), f32(r, c, e), f32(r, t, c)
+    eb, p1, p2, seed = f32(r, c), 0.2, 0.3, 77
+    plan = be.rope_plan(12, layout="half")
+    dev = be.alloc_from_host
+    shape = (b, s, h, d)
+    # forward
+    B, WN = dev(bias), dev(wn)
+    q = be.rope_dev(dev(x), shape, plan, start=5)
+    z = be.dropout_dev(q, B, dev(res), p1, seed, 0, t, c)
+    nrm, rstd = be.rms_norm_dev(z, WN, t, c, 1e-5)
+    nh = be.copy_to_host(nrm).reshape(t, c)
+    logits = nh @ wg
+    logits[4] = -np.inf  # a padded token
+    L = dev(logits)
+    w, ids = be.moe_gate_dev(L, t, e, k)
+    mp = be.moe_sort_dev(ids, t, k, e)
+    with torch.cuda.stream(be.stream):
+        xs = bk().DeviceBuffer(torch.zeros(t * k * c, device=be.device))
+    be.moe_dispatch_dev(nrm, mp, c, out=xs)
+    a = be.bias_act_dev(xs, dev(eb), "silu", t * k, c)
+    m = be.moe_combine_dev(a, w, mp, c)
+    y = be.dropout_dev(m, None, z, p2, seed, be.dropout_counters(t * c), t, c)
+    # backward
+    U = dev(up)
+    dm, _ = be.dropout_backward_dev(U, p2, seed, be.dropout_counters(t * c), t, c)
+    with torch.cuda.stream(be.stream):
+        da = bk().DeviceBuffer(torch.zeros(t * k * c, device=be.device))
+    _, dw = be.moe_combine_backward_dev(dm, a, w, mp, c, dys=da)
+    dxs, deb = be.bias_act_backward_dev(da, xs, dev(eb), "silu", t * k, c)
+    dl = be.moe_gate_backward_dev(dw, L, w, ids, t, e, k)
+    dn = be.moe_dispatch_backward_dev(dxs, mp, c)
+    dn = be.binary_dev(bk().BinaryKind.Add, dn, dev(be.copy_to_host(dl).reshape(t, e) @ wg.T))
+    dz, dwn = be.rms_norm_backward_dev(dn, z, rstd, WN, t, c)
+    dz = be.binary_dev(bk().BinaryKind.Add, dz, U)
+    dq, db = be.dropout_backward_dev(dz, p1, seed, 0, t, c, want_dbias=True)
+    dx = be.rope_backward_dev(dq, shape, plan, start=5)
+    # the same in 64 bits
+    T = lambda v: torch.tensor(np.asarray(v, np.float64), requires_grad=True)
+    tx, tb, tr, twn, twg, teb = (T(v) for v in (x, bias, res, wn, wg, eb))
+    ang = torch.tensor(ref.rope_angles(np.broadcast_to(np.arange(s) + 5, (b, s)), ref.rope_theta(12)))[:, :, None]
+    v = tx.view(shape)
+    f, g2 = v[..., :6], v[..., 6:12]
+    tq = torch.cat([f * ang.cos() - g2 * ang.sin(), g2 * ang.cos() + f * ang.sin(), v[..., 12:]], -1).reshape(t, c)
+    k1 = torch.tensor(ref.drop_keep(t * c, p1, seed, 0).reshape(t, c)) / (1 - float(np.float32(p1)))
+    k2 = torch.tensor(ref.drop_keep(t * c, p2, seed, (t * c + 3) // 4).reshape(t, c)) / (1 - float(np.float32(p2)))
+    tz = (tq + tb) * k1 + tr
+    tn = tz / torch.sqrt((tz * tz).mean(1, keepdim=True) + 1e-5) * twn
+    tl = tn @ twg
+    at = torch.tensor(be.copy_i64_to_host(ids).reshape(t, k))
+    assert (at[4] == -1).all()
+    live = torch.ones(t, 1, dtype=torch.float64)
+    live[4] = 0
+    tw = torch.softmax(tl.gather(1, at.clamp(min=0)), 1) * live
+    top = tl.detach().masked_fill(torch.arange(t)[:, None] == 4, -math.inf)
+    assert (ref.gate(top.numpy(), k, True)[1] == at.numpy()).all()
+    act = torch.nn.functional.silu(tn + teb)
+    tm = (tw[:, :, None] * act[:, None, :]).sum(1)
+    ty = tm * k2 + tz
+    (ty * torch.tensor(up, dtype=torch.float64)).sum().backward()
+    # rms_norm and silu are held to 2e-4 elsewhere; the run multiplies a handful of such errors
+    close = lambda got, want, what: within(be.copy_to_host(got).reshape(want.shape), want.detach().numpy(), 1e-4 * float(want.detach().abs().max()), what)
+    close(y, ty, "y")
+    close(dx, tx.grad, "dx")
+    close(db, tb.grad, "dbias")
+    close(dwn, twn.grad, "dweight")
+    close(dz, tr.grad, "dresidual")
+    # the experts' bias gradient takes the rows of the padded token's places (zeros) along: nothing added
+    close(deb, teb.grad, "dexpert bias")
+
+
+def test_a_captured_step_draws_new_masks_and_equals_eager_calls(be):
+    """The whole run recorded into a CUDA graph and replayed on new inputs: equal to eager calls bit for bit; the device
+    counter makes every replay draw its own mask."""
+    t, e, k, c = 40, 16, 4, 64
+    n = t * c
+    gen = torch.Generator(device=be.device).manual_seed(1)
+    DB = bk().DeviceBuffer
+    with torch.cuda.stream(be.stream):
+        ten = lambda *s_: DB(torch.zeros(*s_, device=be.device).view(-1))
+        x, logits, g = ten(t, c), ten(t, e), ten(t, c)
+        counter = DB(torch.zeros(1, dtype=torch.int64, device=be.device))
+    plan = be.rope_plan(32, layout="interleaved")
+    bufs = {}
+
+    def step():
+        q = be.rope_dev(x, (1, t, 2, 32), plan)
+        z = be.dropout_dev(q, None, x, 0.4, 11, 0, t, c, counter=counter)
+        w, ids = be.moe_gate_dev(logits, t, e, k, renorm=False)
+        mp = be.moe_sort_dev(ids, t, k, e)
+        xs = be.moe_dispatch_dev(z, mp, c)
+        y = be.moe_combine_dev(xs, w, mp, c)
+        dxs, dw = be.moe_combine_backward_dev(g, xs, w, mp, c)
+        dl = be.moe_gate_backward_dev(dw, logits, w, ids, t, e, k, renorm=False)
+        dz = be.moe_dispatch_backward_dev(dxs, mp, c)
+        dq, db = be.dropout_backward_dev(dz, 0.4, 11, 0, t, c, counter=counter, want_dbias=True)
+        dx = be.rope_backward_dev(dq, (1, t, 2, 32), plan)
+        be.dropout_advance_dev(counter, be.dropout_counters(n))
+        return [z, w, ids, mp.place, mp.offsets, xs, y, dw, dl, dz, dq, db, dx]
+
+    step()
+    be.synchronize()
+    counter.t.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=be.stream):
+        bufs["out"] = step()
+    masks = []
+    for trial in range(3):
+        with torch.cuda.stream(be.stream):
+            for v in (x, logits, g):
+                v.t.normal_(generator=gen)
+            counter.t.fill_(trial * n // 4)
+        be.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(counter.t.item()) == (trial + 1) * n // 4
+        from_graph = [o.t.clone() for o in bufs["out"]]
+        masks.append((from_graph[0] == x.t).cpu())
+        counter.t.fill_(trial * n // 4)
+        torch.cuda.synchronize()
+        eager = step()
+        be.synchronize()
+        for i, (a, o) in enumerate(zip(from_graph, eager)):
+            assert torch.equal(a, o.t), (trial, i)
+    assert not torch.equal(masks[0], masks[1]) and not torch.equal(masks[1], masks[2])
+
+
+def test_results_do_not_depend_on_the_run(be):
+    """The same call twice, and on another stream of the same device, gives the same bits: sums have a fixed order."""
+    t, e, k, c = 700, 32, 4, 96
+    r = np.random.default_rng(2)
+    ids, w, ys, dy = r.integers(0, e, t * k), f32(r, t, k), f32(r, t * k, c), f32(r, t, c)
+    from ferro_b200.backend import CudaBackend
+    other = CudaBackend(0)  # a stream of its own
+
+    def all_of(b):
+        plan = b.moe_sort_dev(b.alloc_i64_from_host(ids), t, k, e)
+        y = b.moe_combine_dev(b.alloc_from_host(ys), b.alloc_from_host(w), plan, c)
+        dys, dw = b.moe_combine_backward_dev(b.alloc_from_host(dy), b.alloc_from_host(ys), b.alloc_from_host(w), plan, c)
+        dx, db = b.dropout_backward_dev(b.alloc_from_host(ys), 0.3, 4, 5, t * k, c, want_dbias=True)
+        return [b.copy_to_host(v) for v in (y, dys, dw, dx, db)]
+
+    first = all_of(be)
+    for again in (all_of(be), all_of(other)):
+        assert all((bits(a) == bits(o)).all() for a, o in zip(first, again))
