@@ -6,150 +6,227 @@
 // token ascending), integers are counted with commutative adds only: results do
 // not depend on scheduling.
 #include "common.cuh"
+#include "fastdiv.cuh"
 
 namespace fb {
 
 // ---------------------------------------------------------------- gate
 // One warp per token; lane l holds experts l, l + 32, ...  A logit is turned into
-// an unsigned key whose order is the order of choice: -inf (masked) 0, then the
-// finite values ascending (-0 and +0 equal), +inf, NaN highest.
+// an unsigned key whose order is the order of choice: -inf (masked) lowest, then
+// the finite values ascending, +inf, NaN highest.  Adding +0 first makes -0 and
+// +0 the same key and every NaN the one positive NaN the adder returns.
+constexpr uint32_t kGateMasked = 0x007fffffu;  // the key of -inf
 __device__ __forceinline__ uint32_t gate_key(float v) {
-  if (v != v) return 0xffffffffu;
-  if (v == -INFINITY) return 0u;
-  const uint32_t u = __float_as_uint(v + 0.0f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const int32_t u = __float_as_int(v + 0.0f);
+  return (uint32_t)u ^ ((uint32_t)(u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float gate_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
 constexpr int kGateThreads = 256;
+constexpr int kGateWarps = kGateThreads / 32;
 
+// Choice j of a row for lane j (-1 where there is none): k rounds of a warp-wide maximum over whole
+// keys, then of the lowest index among the lanes that hold it.
 template <int NPL>
+__device__ __forceinline__ int32_t gate_choose_exact(const float* __restrict__ row, uint32_t experts, uint32_t k, int lane) {
+  uint32_t key[NPL];
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) {
+    const uint32_t e = i * 32 + lane;
+    key[i] = e < experts ? gate_key(__ldg(row + e)) : 0u;
+  }
+  int32_t mine = -1;
+  for (uint32_t j = 0; j < k; ++j) {
+    uint32_t lb = 0, li = 0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+      if (key[i] > lb) {
+        lb = key[i];
+        li = i * 32 + lane;
+      }
+    const uint32_t win = __reduce_max_sync(0xffffffffu, lb);
+    if (win <= kGateMasked) break;
+    const uint32_t id = __reduce_min_sync(0xffffffffu, lb == win ? li : 0xffffffffu);
+    if ((uint32_t)lane == j) mine = (int32_t)id;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+      if (i * 32 + lane == id) key[i] = 0;
+  }
+  return mine;
+}
+
+// Sorts a lane's keys, largest first (odd-even transposition: the networks are short).
+template <int NPL>
+__device__ __forceinline__ void gate_sort(uint32_t (&v)[NPL]) {
+#pragma unroll
+  for (int r = 0; r < NPL; ++r)
+#pragma unroll
+    for (int i = r & 1; i + 1 < NPL; i += 2) {
+      const uint32_t hi = max(v[i], v[i + 1]), lo = min(v[i], v[i + 1]);
+      v[i] = hi;
+      v[i + 1] = lo;
+    }
+}
+
+// The same through packed words: the expert's number, complemented, takes the place of the key's lowest
+// IDBITS bits, so that one warp-wide maximum gives value, index and tie-break at once and a lane
+// recognises its own entry by equality.  The order found is exact unless entries that differ only in
+// the bits cut off were met: `ok` is false then, and the caller chooses again with whole keys.  That is
+// the case if two neighbours among the chosen agree in the kept bits but not in value, or if the
+// last chosen and the first left out agree in the kept bits.
+template <int NPL>
+__device__ __forceinline__ int32_t gate_choose_packed(const float* __restrict__ row, const float (&v)[NPL], uint32_t experts,
+                                                      uint32_t k, int lane, float& value, bool& ok) {
+  constexpr uint32_t kIds = 32 * NPL;  // a power of two
+  uint32_t w[NPL];
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) {
+    const uint32_t e = i * 32 + lane;
+    w[i] = e < experts ? (gate_key(v[i]) & ~(kIds - 1)) | (kIds - 1 - e) : 0u;
+  }
+  if constexpr (NPL <= 8) gate_sort(w);
+  uint32_t mine = 0, next = 0;  // next: the first left out
+  for (uint32_t j = 0; j <= k; ++j) {
+    uint32_t head = w[0];
+    if constexpr (NPL > 8) {
+#pragma unroll
+      for (int i = 1; i < NPL; ++i) head = max(head, w[i]);
+    }
+    const uint32_t win = __reduce_max_sync(0xffffffffu, head);
+    if (j == k) {
+      next = win;
+      break;
+    }
+    if ((uint32_t)lane == j) mine = win;
+    if constexpr (NPL <= 8) {
+      if (head == win) {
+#pragma unroll
+        for (int i = 0; i + 1 < NPL; ++i) w[i] = w[i + 1];
+        w[NPL - 1] = 0;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) w[i] = w[i] == win ? 0u : w[i];
+    }
+  }
+  const bool real = mine > kGateMasked;  // lanes from k on hold 0
+  const int32_t id = real ? (int32_t)(kIds - 1 - (mine & (kIds - 1))) : -1;
+  value = real ? __ldg(row + id) + 0.0f : 0.0f;
+  const uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
+  const float after_value = __shfl_down_sync(0xffffffffu, value, 1);
+  bool clash = false;
+  if (real && (uint32_t)lane + 1 < k) clash = (mine & ~(kIds - 1)) == (after & ~(kIds - 1)) && value != after_value && !(value != value && after_value != after_value);
+  if (real && (uint32_t)lane + 1 == k) clash = (mine & ~(kIds - 1)) == (next & ~(kIds - 1));
+  ok = !__any_sync(0xffffffffu, clash);
+  return id;
+}
+
+template <int NPL, bool RENORM>
 __global__ void __launch_bounds__(kGateThreads)
-moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t experts, uint32_t k, int renorm,
+moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t experts, uint32_t k,
                     float* __restrict__ weights, int64_t* __restrict__ ids) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (uint64_t t = (uint64_t)blockIdx.x * (kGateThreads / 32) + warp; t < tokens; t += (uint64_t)gridDim.x * (kGateThreads / 32)) {
-    uint32_t key[NPL];
+  for (uint64_t t = (uint64_t)blockIdx.x * kGateWarps + warp; t < tokens; t += (uint64_t)gridDim.x * kGateWarps) {
+    const float* row = logits + t * experts;
+    float v[NPL];
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const uint32_t e = i * 32 + lane;
-      key[i] = e < experts ? gate_key(__ldg(logits + t * experts + e)) : 0u;
+      v[i] = e < experts ? __ldg(row + e) : -INFINITY;
     }
-    uint32_t best = 0;
+    float value;
+    bool ok;
+    int32_t id = gate_choose_packed<NPL>(row, v, experts, k, lane, value, ok);
+    if (!ok) {
+      id = gate_choose_exact<NPL>(row, experts, k, lane);
+      value = id >= 0 ? __ldg(row + id) : 0.0f;
+    }
+    const float m = __shfl_sync(0xffffffffu, value, 0);  // the largest, where there is one
+    const float mass = id >= 0 ? expf(value - m) : 0.0f;
+    float total;
+    if (RENORM) {
+      total = warp_sum(mass);
+    } else {
+      total = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) best = max(best, key[i]);
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    const float m = gate_value(top);
-    float total = 0.0f;
-    if (!renorm && top) {
-#pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (key[i]) total += expf(gate_value(key[i]) - m);
+      for (int i = 0; i < NPL; ++i) total += v[i] == -INFINITY ? 0.0f : expf(v[i] - m);
       total = warp_sum(total);
     }
-    uint32_t my_key = 0, my_id = 0;  // lane j keeps choice j
-    for (uint32_t j = 0; j < k; ++j) {
-      uint32_t lb = 0, li = 0;
-#pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (key[i] > lb) {
-          lb = key[i];
-          li = i * 32 + lane;
-        }
-      const uint32_t win = __reduce_max_sync(0xffffffffu, lb);
-      if (win == 0) break;
-      const uint32_t id = __reduce_min_sync(0xffffffffu, lb == win ? li : 0xffffffffu);
-      if ((uint32_t)lane == j) {
-        my_key = win;
-        my_id = id;
-      }
-#pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (i * 32 + lane == id) key[i] = 0;
-    }
-    const float mass = my_key ? expf(gate_value(my_key) - m) : 0.0f;
-    const float sum = renorm ? warp_sum(mass) : total;
     if ((uint32_t)lane < k) {
-      weights[t * k + lane] = my_key ? mass / sum : 0.0f;
-      ids[t * k + lane] = my_key ? (int64_t)my_id : -1;
+      weights[t * k + lane] = id >= 0 ? mass / total : 0.0f;
+      ids[t * k + lane] = id;
     }
   }
 }
 
-template <int NPL>
+// Lane j takes choice j; the row is laid out in shared memory, the chosen entries written over it.  A
+// chosen entry is w_j (dw_j - sum w dw) in both forms: the saved weight is its probability.
+template <int NPL, bool RENORM>
 __global__ void __launch_bounds__(kGateThreads)
 moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict__ logits, const float* __restrict__ weights,
-                    const int64_t* __restrict__ ids, uint64_t tokens, uint32_t experts, uint32_t k, int renorm,
+                    const int64_t* __restrict__ ids, uint64_t tokens, uint32_t experts, uint32_t k,
                     float* __restrict__ dlogits) {
+  __shared__ float rows[kGateWarps][32 * NPL];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (uint64_t t = (uint64_t)blockIdx.x * (kGateThreads / 32) + warp; t < tokens; t += (uint64_t)gridDim.x * (kGateThreads / 32)) {
+  float* out = rows[warp];
+  for (uint64_t t = (uint64_t)blockIdx.x * kGateWarps + warp; t < tokens; t += (uint64_t)gridDim.x * kGateWarps) {
     float w = 0.0f, dw = 0.0f;
-    uint32_t id = 0xffffffffu;
+    int64_t id = -1;
     if ((uint32_t)lane < k) {
-      const int64_t e = __ldg(ids + t * k + lane);
-      if (e >= 0 && e < (int64_t)experts) {
-        id = (uint32_t)e;
+      id = __ldg(ids + t * k + lane);
+      if (id < 0 || id >= (int64_t)experts) id = -1;
+      else {
         w = __ldg(weights + t * k + lane);
         dw = __ldg(dweights + t * k + lane);
       }
     }
-    const float dot = warp_sum(w * dw);
-    float p[NPL], acc[NPL];
-    if (!renorm) {
-      uint32_t best = 0;
+    float p[NPL];
+    if (!RENORM) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         const uint32_t e = i * 32 + lane;
-        const float v = e < experts ? __ldg(logits + t * experts + e) : -INFINITY;
-        p[i] = v;
-        best = max(best, gate_key(v));
+        p[i] = e < experts ? __ldg(logits + t * experts + e) : -INFINITY;
       }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-      const float m = gate_value(top);
+    }
+    const float dot = warp_sum(w * dw);
+    if (!RENORM) {
+      uint32_t best = gate_key(p[0]);
+#pragma unroll
+      for (int i = 1; i < NPL; ++i) best = max(best, gate_key(p[i]));
+      const float m = gate_value(__reduce_max_sync(0xffffffffu, best));
       float total = 0.0f;
-      uint32_t live = 0;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        const bool on = p[i] != -INFINITY;
-        live |= (uint32_t)on << i;
-        p[i] = on ? expf(p[i] - m) : 0.0f;
+        p[i] = p[i] == -INFINITY ? -0.0f : expf(p[i] - m);  // -0: masked, stays 0 whatever total is
         total += p[i];
       }
       total = warp_sum(total);
+      const float f = -dot / total;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) {
-        p[i] = (live >> i) & 1 ? p[i] / total : 0.0f;
-        acc[i] = -p[i] * dot;
-      }
+      for (int i = 0; i < NPL; ++i) out[i * 32 + lane] = __float_as_uint(p[i]) == 0x80000000u ? 0.0f : p[i] * f;
     } else {
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) acc[i] = 0.0f;
+      for (int i = 0; i < NPL; ++i) out[i * 32 + lane] = 0.0f;
     }
-    for (uint32_t j = 0; j < k; ++j) {
-      const uint32_t e = __shfl_sync(0xffffffffu, id, j);
-      const float wj = __shfl_sync(0xffffffffu, w, j), dwj = __shfl_sync(0xffffffffu, dw, j);
-      if (e == 0xffffffffu) continue;
-#pragma unroll
-      for (int i = 0; i < NPL; ++i)
-        if (i * 32 + lane == e) acc[i] = renorm ? wj * (dwj - dot) : p[i] * (dwj - dot);
-    }
+    __syncwarp();
+    if (id >= 0) out[id] = w * (dw - dot);
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const uint32_t e = i * 32 + lane;
-      if (e < experts) dlogits[t * experts + e] = acc[i];
+      if (e < experts) dlogits[t * experts + e] = out[e];
     }
+    __syncwarp();
   }
 }
 
 // ---------------------------------------------------------------- sort
-// Counting sort.  A CTA owns kSortChunk neighbouring assignments, a warp 32 *
-// kSortRounds of them.  Within a warp the rank of an assignment among those of
-// its expert comes from the lanes that hold the same id (match) plus the warp's
-// running count; between warps and CTAs counts are summed in order.
+// Counting sort.  A CTA owns a chunk of neighbouring assignments, a warp 32 * R of them.  Within a
+// warp the rank of an assignment among those of its expert comes from the lanes that hold the same id
+// (match) plus the warp's running count; between warps and chunks counts are summed in order.
 constexpr int kSortThreads = 1024;
-constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortRounds = 4;
 constexpr uint32_t kSortChunk = kSortThreads * kSortRounds;
 
@@ -160,18 +237,20 @@ __device__ __forceinline__ uint32_t sort_id(int64_t e, uint32_t experts) {
 // counts[b][e] = how many assignments of chunk b go to expert e.
 __global__ void __launch_bounds__(kSortThreads)
 moe_count_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, uint32_t* __restrict__ counts) {
+  pdl_trigger();
   extern __shared__ uint32_t hist[];
-  for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) hist[e] = 0;
-  __syncthreads();
   const uint32_t base = blockIdx.x * kSortChunk;
+  uint32_t id[kSortRounds];
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
     const uint32_t i = base + r * kSortThreads + threadIdx.x;
-    if (i < n) {
-      const uint32_t e = sort_id(__ldg(ids + i), experts);
-      if (e < experts) atomicAdd(&hist[e], 1u);
-    }
+    id[r] = i < n ? sort_id(__ldg(ids + i), experts) : experts;
   }
+  for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) hist[e] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r)
+    if (id[r] < experts) atomicAdd(&hist[id[r]], 1u);
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) counts[(uint64_t)blockIdx.x * experts + e] = hist[e];
 }
@@ -180,6 +259,8 @@ moe_count_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
 // number in all.  A CTA owns 32 experts (lanes) and splits the chunks into 32 runs (warps).
 __global__ void __launch_bounds__(1024)
 moe_scan_kernel(uint32_t* __restrict__ counts, uint32_t chunks, uint32_t experts, uint32_t* __restrict__ totals) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ uint32_t part[32][33];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
   const uint32_t run = (chunks + 31) / 32, lo = min(chunks, warp * run), hi = min(chunks, lo + run);
@@ -205,25 +286,25 @@ moe_scan_kernel(uint32_t* __restrict__ counts, uint32_t chunks, uint32_t experts
 enum { SORT_ALONE = 0, SORT_DIRECT = 1, SORT_SCANNED = 2 };
 constexpr uint32_t kSortDirect = 64;
 
-__global__ void __launch_bounds__(kSortThreads)
+// blockDim.x is a multiple of 32 and at least `experts`.
+template <int R>
+__global__ void __launch_bounds__(kSortThreads, 1)
 moe_place_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, uint32_t chunks, int mode,
-                 const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals, int64_t* __restrict__ place, int64_t* __restrict__ order,
-                 int64_t* __restrict__ offsets, int64_t* __restrict__ bad) {
+                 const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals, int64_t* __restrict__ place,
+                 int64_t* __restrict__ order, int64_t* __restrict__ offsets, int64_t* __restrict__ bad) {
   extern __shared__ uint32_t sm[];
-  uint32_t* total = sm;                // [experts + 1] over all chunks, then first rows
-  uint32_t* before = total + experts + 1;  // [experts] in the chunks before this one
-  uint32_t* hist = before + experts;   // [warps][experts]
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const uint32_t stride = experts | 1;  // odd: a column of hist touches every bank
+  uint32_t* total = sm;                 // [experts] over all chunks, then first rows
+  uint32_t* before = total + experts;   // [experts] in the chunks before this one
+  uint32_t* hist = before + experts;    // [warps][stride]
   __shared__ uint32_t wsum[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (uint32_t i = threadIdx.x; i < kSortWarps * experts; i += kSortThreads) hist[i] = 0;
-  for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) total[e] = before[e] = 0;
-  __syncthreads();
-  // ranks within the warp
-  const uint32_t base = blockIdx.x * kSortChunk + warp * 32 * kSortRounds + lane;
-  uint32_t id[kSortRounds], rank[kSortRounds];
-  uint32_t* mine = hist + warp * experts;
+  // The ids are older than the kernel before this one (moe_count_kernel only reads them, and started
+  // after whatever wrote them had ended): they may be read before pdl_wait.
+  const uint32_t base = blockIdx.x * (blockDim.x * R) + warp * 32 * R + lane;
+  uint32_t id[R], rank[R];
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const uint32_t i = base + r * 32;
     id[r] = experts;
     if (i < n) {
@@ -232,69 +313,78 @@ moe_place_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
       if (id[r] == experts && e != -1 && bad) atomicMax(reinterpret_cast<long long*>(bad), (long long)i + 1);
     }
   }
+  for (uint32_t i = threadIdx.x; i < warps * stride; i += blockDim.x) hist[i] = 0;
+  for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) total[e] = before[e] = 0;
+  __syncthreads();
+  // ranks within the warp
+  uint32_t* mine = hist + warp * stride;
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const uint32_t same = __match_any_sync(0xffffffffu, id[r]);
     const uint32_t old = id[r] < experts ? mine[id[r]] : 0u;
     rank[r] = old + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
-    if (id[r] < experts && lane == __ffs(same) - 1) mine[id[r]] = old + __popc(same);
+    if (id[r] < experts && lane == (uint32_t)__ffs(same) - 1) mine[id[r]] = old + __popc(same);
     __syncwarp();
   }
-  __syncthreads();
-  // exclusive prefix over the warps of this CTA; its total
-  for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) {
-    uint32_t acc = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = hist[w * experts + e];
-      hist[w * experts + e] = acc;
-      acc += c;
-    }
-    if (mode == SORT_ALONE) total[e] = acc;
-    if (mode == SORT_SCANNED) {
-      total[e] = totals[e];
-      before[e] = counts[(uint64_t)blockIdx.x * experts + e];
-    }
-  }
+  if (mode != SORT_ALONE) pdl_wait();
   if (mode == SORT_DIRECT) {
-    for (uint64_t i = threadIdx.x; i < (uint64_t)chunks * experts; i += kSortThreads) {
-      const uint32_t b = (uint32_t)(i / experts), e = (uint32_t)(i - (uint64_t)b * experts);
-      const uint32_t c = __ldg(counts + i);
-      if (c) {
-        atomicAdd(&total[e], c);
-        if (b < blockIdx.x) atomicAdd(&before[e], c);
+    // groups of `experts` threads take the chunks in turn
+    const uint32_t groups = blockDim.x / experts, g = threadIdx.x / experts, e = threadIdx.x - g * experts;
+    if (g < groups) {
+      uint32_t all = 0, pre = 0;
+      for (uint32_t b = g; b < chunks; b += groups) {
+        const uint32_t c = __ldcg(counts + (uint64_t)b * experts + e);
+        all += c;
+        if (b < blockIdx.x) pre += c;
       }
+      atomicAdd(&total[e], all);
+      atomicAdd(&before[e], pre);
     }
+  } else if (mode == SORT_SCANNED && threadIdx.x < experts) {
+    total[threadIdx.x] = __ldcg(totals + threadIdx.x);
+    before[threadIdx.x] = __ldcg(counts + (uint64_t)blockIdx.x * experts + threadIdx.x);
+  }
+  __syncthreads();
+  // exclusive prefix over the warps of this CTA: a warp per expert, lanes along the warps
+  for (uint32_t e = warp; e < experts; e += warps) {
+    const uint32_t c = lane < warps ? hist[lane * stride + e] : 0u;
+    uint32_t inc = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= (uint32_t)o) inc += up;
+    }
+    if (lane < warps) hist[lane * stride + e] = inc - c;
+    if (lane == 31 && mode == SORT_ALONE) total[e] = inc;
   }
   __syncthreads();
   // exclusive scan over the experts (at most one per thread)
-  uint32_t v = threadIdx.x < experts ? total[threadIdx.x] : 0u, inc = v;
+  const uint32_t v = threadIdx.x < experts ? total[threadIdx.x] : 0u;
+  uint32_t inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t up = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += up;
+    if (lane >= (uint32_t)o) inc += up;
   }
   if (lane == 31) wsum[warp] = inc;
   __syncthreads();
-  if (warp == 0) {
-    uint32_t s = wsum[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += up;
-    }
-    wsum[lane] = s;
+  uint32_t lower = 0;  // what the warps below hold
+  {
+    uint32_t s = lane < warp ? wsum[lane] : 0u;
+    lower = __reduce_add_sync(0xffffffffu, s);
   }
-  __syncthreads();
-  const uint32_t excl = inc - v + (warp ? wsum[warp - 1] : 0u);
+  const uint32_t excl = inc - v + lower;
   if (threadIdx.x < experts) {
     total[threadIdx.x] = excl + before[threadIdx.x];
-    if (blockIdx.x == 0) offsets[threadIdx.x] = excl;
+    if (blockIdx.x == 0) {
+      offsets[threadIdx.x] = excl;
+      if (threadIdx.x + 1 == experts) offsets[experts] = excl + v;
+    }
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) offsets[experts] = wsum[kSortWarps - 1];
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const uint32_t i = base + r * 32;
     if (i >= n) continue;
     int64_t at = -1;
@@ -307,104 +397,176 @@ moe_place_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
 }
 
 // ---------------------------------------------------------------- rows
-// A token is owned by TPT threads (a power of two from 32 to 256); a thread walks the columns in
-// vectors of VEC floats.
 constexpr int kRowThreads = 256;
 
 template <int VEC>
-struct RowVec;
-template <>
-struct RowVec<4> {
-  using T = float4;
-  static __device__ __forceinline__ T load(const float* p) { return ld_stream4(p); }
-  static __device__ __forceinline__ void store(float* p, T v) { st_stream4(p, v); }
-  static __device__ __forceinline__ T zero() { return make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
-  static __device__ __forceinline__ T mul(T a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
-  static __device__ __forceinline__ T add(T a, T b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
-  static __device__ __forceinline__ T fma(T a, float s, T c) {
-    return make_float4(fmaf(a.x, s, c.x), fmaf(a.y, s, c.y), fmaf(a.z, s, c.z), fmaf(a.w, s, c.w));
+struct RowVec {
+  static_assert(VEC == 1 || VEC == 2 || VEC == 4, "floats of one access");
+  float v[VEC];
+  __device__ __forceinline__ void load(const float* p) {
+    if constexpr (VEC == 4) {
+      const float4 t = ld_stream4(p);
+      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    } else if constexpr (VEC == 2) {
+      const float2 t = __ldcs(reinterpret_cast<const float2*>(p));
+      v[0] = t.x; v[1] = t.y;
+    } else {
+      v[0] = ld_stream(p);
+    }
   }
-  static __device__ __forceinline__ float dot(T a, T b, float c) {
-    return fmaf(a.w, b.w, fmaf(a.z, b.z, fmaf(a.y, b.y, fmaf(a.x, b.x, c))));
+  __device__ __forceinline__ void store(float* p) const {
+    if constexpr (VEC == 4) st_stream4(p, make_float4(v[0], v[1], v[2], v[3]));
+    else if constexpr (VEC == 2) __stcs(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
+    else st_stream(p, v[0]);
   }
 };
-template <>
-struct RowVec<1> {
-  using T = float;
-  static __device__ __forceinline__ T load(const float* p) { return ld_stream(p); }
-  static __device__ __forceinline__ void store(float* p, T v) { st_stream(p, v); }
-  static __device__ __forceinline__ T zero() { return 0.0f; }
-  static __device__ __forceinline__ T mul(T a, float s) { return a * s; }
-  static __device__ __forceinline__ T add(T a, T b) { return a + b; }
-  static __device__ __forceinline__ T fma(T a, float s, T c) { return fmaf(a, s, c); }
-  static __device__ __forceinline__ float dot(T a, T b, float c) { return fmaf(a, b, c); }
+
+// Where a thread stands: a token's row is cut into vectors, a CTA takes `tpb` whole tokens or one of
+// `bpt` pieces of a token, a thread one vector.
+struct RowMap {
+  uint64_t tokens, cols, slots, blocks;
+  uint32_t k, vpt;    // vectors per row
+  uint32_t tpb, bpt;
+  FastDiv d_vpt;
 };
+__device__ __forceinline__ bool row_place(const RowMap& M, uint64_t blk, uint64_t& t, uint32_t& vec) {
+  if (M.bpt == 1) {
+    const uint32_t tl = fdiv(threadIdx.x, M.d_vpt);
+    vec = threadIdx.x - tl * M.vpt;
+    t = blk * M.tpb + tl;
+    return tl < M.tpb && t < M.tokens;
+  }
+  t = blk / M.bpt;
+  vec = (uint32_t)(blk - t * M.bpt) * kRowThreads + threadIdx.x;
+  return vec < M.vpt;
+}
 
 __device__ __forceinline__ int64_t slot_of(const int64_t* place, uint64_t a, uint64_t slots) {
   const int64_t s = __ldg(place + a);
   return s >= 0 && (uint64_t)s < slots ? s : -1;
 }
 
-// xs[place[t, j]] = x[t]
-template <int VEC>
+// xs[place[t, j]] = x[t], KU choices at a time: their places are loaded before the first store.
+template <int VEC, int KU>
 __global__ void __launch_bounds__(kRowThreads)
-moe_scatter_kernel(const float* __restrict__ x, const int64_t* __restrict__ place, uint64_t tokens, uint32_t k,
-                   uint64_t cols, uint64_t slots, uint32_t tpt, float* __restrict__ xs) {
-  using R = RowVec<VEC>;
-  const uint32_t per_cta = kRowThreads / tpt, mine = threadIdx.x / tpt, l = threadIdx.x % tpt;
-  for (uint64_t t = (uint64_t)blockIdx.x * per_cta + mine; t < tokens; t += (uint64_t)gridDim.x * per_cta)
-    for (uint64_t c = (uint64_t)l * VEC; c < cols; c += (uint64_t)tpt * VEC) {
-      const typename R::T v = R::load(x + t * cols + c);
-      for (uint32_t j = 0; j < k; ++j) {
-        const int64_t s = slot_of(place, t * k + j, slots);
-        if (s >= 0) R::store(xs + (uint64_t)s * cols + c, v);
-      }
+moe_scatter_kernel(const float* __restrict__ x, const int64_t* __restrict__ place, const __grid_constant__ RowMap M,
+                   float* __restrict__ xs) {
+  for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
+    uint64_t t;
+    uint32_t vec;
+    if (!row_place(M, blk, t, vec)) continue;
+    const uint64_t c = (uint64_t)vec * VEC;
+    RowVec<VEC> v;
+    v.load(x + t * M.cols + c);
+    for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
+      int64_t s[KU];
+#pragma unroll
+      for (int j = 0; j < KU; ++j) s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
+#pragma unroll
+      for (int j = 0; j < KU; ++j)
+        if (s[j] >= 0) v.store(xs + (uint64_t)s[j] * M.cols + c);
     }
+  }
 }
 
-// y[t] = sum over j of (weights[t, j] *) ys[place[t, j]]
-template <int VEC, bool WEIGHTED>
+// y[t] = sum over j of (weights[t, j] *) ys[place[t, j]], KU rows in flight, added in the order of j.
+template <int VEC, int KU, bool WEIGHTED>
 __global__ void __launch_bounds__(kRowThreads)
 moe_gather_kernel(const float* __restrict__ ys, const float* __restrict__ weights, const int64_t* __restrict__ place,
-                  uint64_t tokens, uint32_t k, uint64_t cols, uint64_t slots, uint32_t tpt, float* __restrict__ y) {
-  using R = RowVec<VEC>;
-  const uint32_t per_cta = kRowThreads / tpt, mine = threadIdx.x / tpt, l = threadIdx.x % tpt;
-  for (uint64_t t = (uint64_t)blockIdx.x * per_cta + mine; t < tokens; t += (uint64_t)gridDim.x * per_cta)
-    for (uint64_t c = (uint64_t)l * VEC; c < cols; c += (uint64_t)tpt * VEC) {
-      typename R::T acc = R::zero();
-      for (uint32_t j = 0; j < k; ++j) {
-        const int64_t s = slot_of(place, t * k + j, slots);
-        if (s < 0) continue;
-        const typename R::T v = R::load(ys + (uint64_t)s * cols + c);
-        acc = WEIGHTED ? R::fma(v, __ldg(weights + t * k + j), acc) : R::add(acc, v);
+                  const __grid_constant__ RowMap M, float* __restrict__ y) {
+  for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
+    uint64_t t;
+    uint32_t vec;
+    if (!row_place(M, blk, t, vec)) continue;
+    const uint64_t c = (uint64_t)vec * VEC;
+    RowVec<VEC> acc;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc.v[i] = 0.0f;
+    for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
+      int64_t s[KU];
+      float w[KU];
+#pragma unroll
+      for (int j = 0; j < KU; ++j) {
+        s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
+        if (WEIGHTED) w[j] = j0 + j < M.k ? __ldg(weights + t * M.k + j0 + j) : 0.0f;
       }
-      R::store(y + t * cols + c, acc);
+      RowVec<VEC> r[KU];
+#pragma unroll
+      for (int j = 0; j < KU; ++j)
+        if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * M.cols + c);
+#pragma unroll
+      for (int j = 0; j < KU; ++j)
+        if (s[j] >= 0) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) acc.v[i] = WEIGHTED ? fmaf(r[j].v[i], w[j], acc.v[i]) : acc.v[i] + r[j].v[i];
+        }
     }
+    acc.store(y + t * M.cols + c);
+  }
 }
 
-// dys[place[t, j]] = weights[t, j] * dy[t]; dweights[t, j] = dy[t] . ys[place[t, j]].  One CTA per token.
-template <int VEC>
-__global__ void __launch_bounds__(kRowThreads)
+// dys[place[t, j]] = weights[t, j] * dy[t]; dweights[t, j] = dy[t] . ys[place[t, j]].  A token is owned by
+// a warp (WARP) or by the CTA, which walks the columns with KU rows of ys in flight; dy is read once per KU choices.
+// dys may be ys: an element is read by the thread that writes it, before it does.
+template <int VEC, int KU, bool WARP>
+__global__ void __launch_bounds__(kRowThreads, KU == 8 ? 2 : 3)
 moe_combine_bwd_kernel(const float* __restrict__ dy, const float* ys, const float* __restrict__ weights,
                        const int64_t* __restrict__ place, uint64_t tokens, uint32_t k, uint64_t cols, uint64_t slots,
                        float* dys, float* __restrict__ dweights) {
-  using R = RowVec<VEC>;
-  __shared__ float red[32];
-  for (uint64_t t = blockIdx.x; t < tokens; t += gridDim.x)
-    for (uint32_t j = 0; j < k; ++j) {
-      const int64_t s = slot_of(place, t * k + j, slots);
-      float dot = 0.0f;
-      if (s >= 0) {
-        const float w = __ldg(weights + t * k + j);
-        for (uint64_t c = (uint64_t)threadIdx.x * VEC; c < cols; c += (uint64_t)kRowThreads * VEC) {
-          const typename R::T g = R::load(dy + t * cols + c);
-          if (dweights) dot = R::dot(g, R::load(ys + (uint64_t)s * cols + c), dot);
-          if (dys) R::store(dys + (uint64_t)s * cols + c, R::mul(g, w));
+  __shared__ float part[kRowThreads / 32][KU];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const uint64_t first = WARP ? (uint64_t)blockIdx.x * warps + warp : blockIdx.x;
+  const uint64_t step = WARP ? (uint64_t)gridDim.x * warps : gridDim.x;
+  const uint32_t l = WARP ? lane : threadIdx.x, width = WARP ? 32 : blockDim.x;
+  for (uint64_t t = first; t < tokens; t += step)
+    for (uint32_t j0 = 0; j0 < k; j0 += KU) {
+      int64_t s[KU];
+      float w[KU], dot[KU];
+#pragma unroll
+      for (int j = 0; j < KU; ++j) {
+        s[j] = j0 + j < k ? slot_of(place, t * k + j0 + j, slots) : -1;
+        w[j] = j0 + j < k ? __ldg(weights + t * k + j0 + j) : 0.0f;
+        dot[j] = 0.0f;
+      }
+      for (uint64_t c = (uint64_t)l * VEC; c < cols; c += (uint64_t)width * VEC) {
+        RowVec<VEC> g, r[KU];
+        g.load(dy + t * cols + c);
+        if (dweights) {
+#pragma unroll
+          for (int j = 0; j < KU; ++j)
+            if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * cols + c);
+#pragma unroll
+          for (int j = 0; j < KU; ++j)
+            if (s[j] >= 0) {
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) dot[j] = fmaf(g.v[i], r[j].v[i], dot[j]);
+            }
+        }
+        if (dys) {
+#pragma unroll
+          for (int j = 0; j < KU; ++j)
+            if (s[j] >= 0) {
+              RowVec<VEC> o;
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) o.v[i] = g.v[i] * w[j];
+              o.store(dys + (uint64_t)s[j] * cols + c);
+            }
         }
       }
-      if (dweights) {
-        dot = block_sum(dot, red);
-        if (threadIdx.x == 0) dweights[t * k + j] = dot;
+      if (!dweights) continue;
+      const float sum = lanes_transpose_sum<32, KU>(dot, lane);  // choice lane / (32 / KU)
+      const uint32_t mine = lane / (32 / KU);
+      if (WARP) {
+        if (lane % (32 / KU) == 0 && j0 + mine < k) dweights[t * k + j0 + mine] = sum;
+      } else {
+        if (lane % (32 / KU) == 0) part[warp][mine] = sum;
+        __syncthreads();
+        if (threadIdx.x < KU && j0 + threadIdx.x < k) {
+          float all = 0.0f;
+          for (uint32_t i = 0; i < warps; ++i) all += part[i][threadIdx.x];
+          dweights[t * k + j0 + threadIdx.x] = all;
+        }
+        __syncthreads();
       }
     }
 }
@@ -425,16 +587,39 @@ static int rows_check(const char* name, uint64_t tokens, uint64_t k, uint64_t co
   if (mul_overflows(tokens, k, &n) || n > (UINT64_MAX >> 4) || mul_overflows(tokens, cols, &n) || n > (UINT64_MAX >> 3) ||
       mul_overflows(slots, cols, &n) || n > (UINT64_MAX >> 3))
     return fail(FB_ERR_INVALID_SHAPE, "%s: size overflow", name);
+  if (cols >= (1ull << 31)) return fail(FB_ERR_UNSUPPORTED, "%s: rows of 2^31 or more elements are not supported", name);
   return FB_OK;
 }
 
-static uint32_t threads_per_token(uint64_t vecs) {
-  uint32_t t = 32;
-  while (t < kRowThreads && t < vecs) t <<= 1;
-  return t;
+static RowMap row_map(uint64_t tokens, uint64_t k, uint64_t cols, uint64_t slots, int vec) {
+  RowMap m = {};
+  m.tokens = tokens;
+  m.cols = cols;
+  m.slots = slots;
+  m.k = (uint32_t)k;
+  m.vpt = (uint32_t)(cols / vec);
+  m.tpb = m.vpt < kRowThreads ? kRowThreads / m.vpt : 1;
+  m.bpt = (m.vpt + kRowThreads - 1) / kRowThreads;
+  m.d_vpt = make_fastdiv(m.vpt);
+  m.blocks = (tokens + m.tpb - 1) / m.tpb * m.bpt;
+  return m;
 }
 
-// f(std::integral_constant<int, NPL>) for the number of experts a lane holds.
+// Floats of one access: as many of 4, 2, 1 as the row length and both addresses allow.
+static int row_vec(uint64_t cols, const void* a, const void* b, const void* c = nullptr) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c);
+  return cols % 4 == 0 && at % 16 == 0 ? 4 : cols % 2 == 0 && at % 8 == 0 ? 2 : 1;
+}
+
+// CALL(VEC, KU) for the access width and the number of choices taken at a time.
+#define FB_ROW_DISPATCH(vec, k, CALL)                             \
+  do {                                                            \
+    if ((vec) == 4) { if ((k) <= 2) { CALL(4, 2); } else if ((k) <= 4) { CALL(4, 4); } else { CALL(4, 8); } } \
+    else if ((vec) == 2) { if ((k) <= 2) { CALL(2, 2); } else if ((k) <= 4) { CALL(2, 4); } else { CALL(2, 8); } } \
+    else { if ((k) <= 2) { CALL(1, 2); } else if ((k) <= 4) { CALL(1, 4); } else { CALL(1, 8); } } \
+  } while (0)
+
+// CALL(NPL) for the number of experts a lane holds.
 #define FB_GATE_DISPATCH(experts, CALL)            \
   do {                                             \
     if ((experts) <= 32) { CALL(1); }              \
@@ -460,8 +645,9 @@ int fb_moe_gate_fwd(fb_stream_t stream, const float* logits, uint64_t tokens, ui
   if (tokens == 0) return FB_OK;
   if (!logits || !weights || !ids) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   const unsigned grid = grid_full((tokens + kGateThreads / 32 - 1) / (kGateThreads / 32));
-#define FB_CALL(NPL) \
-  moe_gate_fwd_kernel<NPL><<<grid, kGateThreads, 0, stream>>>(logits, tokens, (uint32_t)experts, (uint32_t)k, renorm != 0, weights, ids)
+#define FB_CALL(NPL)                                                                                                          \
+  if (renorm) moe_gate_fwd_kernel<NPL, true><<<grid, kGateThreads, 0, stream>>>(logits, tokens, (uint32_t)experts, (uint32_t)k, weights, ids); \
+  else moe_gate_fwd_kernel<NPL, false><<<grid, kGateThreads, 0, stream>>>(logits, tokens, (uint32_t)experts, (uint32_t)k, weights, ids)
   FB_GATE_DISPATCH(experts, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
@@ -475,9 +661,9 @@ int fb_moe_gate_bwd(fb_stream_t stream, const float* dweights, const float* logi
   if (tokens == 0) return FB_OK;
   if (!dweights || !weights || !ids || !dlogits || (!renorm && !logits)) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   const unsigned grid = grid_full((tokens + kGateThreads / 32 - 1) / (kGateThreads / 32));
-#define FB_CALL(NPL)                                                                                               \
-  moe_gate_bwd_kernel<NPL><<<grid, kGateThreads, 0, stream>>>(dweights, logits, weights, ids, tokens, (uint32_t)experts, \
-                                                              (uint32_t)k, renorm != 0, dlogits)
+#define FB_CALL(NPL)                                                                                                          \
+  if (renorm) moe_gate_bwd_kernel<NPL, true><<<grid, kGateThreads, 0, stream>>>(dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, dlogits); \
+  else moe_gate_bwd_kernel<NPL, false><<<grid, kGateThreads, 0, stream>>>(dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, dlogits)
   FB_GATE_DISPATCH(experts, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
@@ -500,21 +686,30 @@ int fb_moe_sort(fb_stream_t stream, const int64_t* ids, uint64_t n, uint64_t exp
   const uint64_t need = fb_moe_sort_workspace_bytes(n, experts);
   if (need && (!workspace || workspace_bytes < need))
     return fail(FB_ERR_WORKSPACE, "%s: needs %llu bytes of scratch", name, (unsigned long long)need);
-  const uint32_t chunks = n ? sort_chunks(n) : 1, E = (uint32_t)experts;
-  const size_t smem = (2 * (size_t)E + 1 + (size_t)kSortWarps * E) * sizeof(uint32_t);
-  if (smem > 48 * 1024) FB_CUDA(allow_dyn_smem((const void*)moe_place_kernel, smem));
+  const uint32_t chunks = n ? sort_chunks(n) : 1, E = (uint32_t)experts, n32 = (uint32_t)n;
+  // One CTA with a thread per assignment where that suffices, else kSortRounds per thread.
+  const bool small = n <= kSortThreads;
+  const uint32_t most = n32 > E ? n32 : E, threads = small ? (most + 31) / 32 * 32 : kSortThreads;
+  const size_t smem = (2 * (size_t)E + (size_t)(threads / 32) * (E | 1)) * sizeof(uint32_t);
+  const void* kernel = small ? (const void*)moe_place_kernel<1> : (const void*)moe_place_kernel<kSortRounds>;
+  if (smem > 48 * 1024) FB_CUDA(allow_dyn_smem(kernel, smem));
   uint32_t* counts = static_cast<uint32_t*>(workspace);
   uint32_t* totals = counts + (uint64_t)chunks * E;
   const int mode = chunks == 1 ? SORT_ALONE : chunks <= kSortDirect ? SORT_DIRECT : SORT_SCANNED;
-  if (chunks > 1) {
-    moe_count_kernel<<<chunks, kSortThreads, E * sizeof(uint32_t), stream>>>(ids, (uint32_t)n, E, counts);
+  if (mode == SORT_ALONE) {
+    if (small) moe_place_kernel<1><<<1, threads, smem, stream>>>(ids, n32, E, 1, mode, nullptr, nullptr, place, order, offsets, bad_index);
+    else moe_place_kernel<kSortRounds><<<1, threads, smem, stream>>>(ids, n32, E, 1, mode, nullptr, nullptr, place, order, offsets, bad_index);
     FB_LAUNCHED(name);
+    return FB_OK;
   }
+  moe_count_kernel<<<chunks, kSortThreads, E * sizeof(uint32_t), stream>>>(ids, n32, E, counts);
+  FB_LAUNCHED(name);
   if (mode == SORT_SCANNED) {
-    moe_scan_kernel<<<(E + 31) / 32, 1024, 0, stream>>>(counts, chunks, E, totals);
+    FB_CUDA(launch_pdl(moe_scan_kernel, dim3((E + 31) / 32), dim3(1024), 0, stream, counts, chunks, E, totals));
     FB_LAUNCHED(name);
   }
-  moe_place_kernel<<<chunks, kSortThreads, smem, stream>>>(ids, (uint32_t)n, E, chunks, mode, counts, totals, place, order, offsets, bad_index);
+  FB_CUDA(launch_pdl(moe_place_kernel<kSortRounds>, dim3(chunks), dim3(threads), smem, stream, ids, n32, E, chunks, mode,
+                     (const uint32_t*)counts, (const uint32_t*)totals, place, order, offsets, bad_index));
   FB_LAUNCHED(name);
   return FB_OK;
 }
@@ -526,11 +721,12 @@ int fb_moe_dispatch_fwd(fb_stream_t stream, const float* x, const int64_t* place
   if (tokens == 0 || cols == 0 || slots == 0) return FB_OK;
   if (!x || !place || !xs) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (xs == x) return fail(FB_ERR_INVALID_ARG, "%s: xs must not be x", name);
-  const bool vec = cols % 4 == 0 && aligned16(x) && aligned16(xs);
-  const uint32_t tpt = threads_per_token(vec ? cols / 4 : cols);
-  const unsigned grid = grid_full((tokens + kRowThreads / tpt - 1) / (kRowThreads / tpt));
-  if (vec) moe_scatter_kernel<4><<<grid, kRowThreads, 0, stream>>>(x, place, tokens, (uint32_t)k, cols, slots, tpt, xs);
-  else moe_scatter_kernel<1><<<grid, kRowThreads, 0, stream>>>(x, place, tokens, (uint32_t)k, cols, slots, tpt, xs);
+  const int vec = row_vec(cols, x, xs);
+  const RowMap m = row_map(tokens, k, cols, slots, vec);
+  const unsigned grid = grid_full(m.blocks);
+#define FB_CALL(VEC, KU) moe_scatter_kernel<VEC, KU><<<grid, kRowThreads, 0, stream>>>(x, place, m, xs)
+  FB_ROW_DISPATCH(vec, k, FB_CALL);
+#undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
 }
@@ -541,16 +737,14 @@ static int gather_rows(cudaStream_t stream, const char* name, const float* ys, c
   if (tokens == 0 || cols == 0) return FB_OK;
   if ((slots && !ys) || !place || !y) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (ys == y) return fail(FB_ERR_INVALID_ARG, "%s: the output must not be the input", name);
-  const bool vec = cols % 4 == 0 && aligned16(ys) && aligned16(y);
-  const uint32_t tpt = threads_per_token(vec ? cols / 4 : cols), k32 = (uint32_t)k;
-  const unsigned grid = grid_full((tokens + kRowThreads / tpt - 1) / (kRowThreads / tpt));
-  if (weights) {
-    if (vec) moe_gather_kernel<4, true><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, tokens, k32, cols, slots, tpt, y);
-    else moe_gather_kernel<1, true><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, tokens, k32, cols, slots, tpt, y);
-  } else {
-    if (vec) moe_gather_kernel<4, false><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, tokens, k32, cols, slots, tpt, y);
-    else moe_gather_kernel<1, false><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, tokens, k32, cols, slots, tpt, y);
-  }
+  const int vec = row_vec(cols, ys, y);
+  const RowMap m = row_map(tokens, k, cols, slots, vec);
+  const unsigned grid = grid_full(m.blocks);
+#define FB_CALL(VEC, KU)                                                                                            \
+  if (weights) moe_gather_kernel<VEC, KU, true><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, m, y);        \
+  else moe_gather_kernel<VEC, KU, false><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, m, y)
+  FB_ROW_DISPATCH(vec, k, FB_CALL);
+#undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
 }
@@ -574,10 +768,18 @@ int fb_moe_combine_bwd(fb_stream_t stream, const float* dy, const float* ys, con
   if (cols == 0) return dweights ? fb_fill(stream, dweights, 0.0f, tokens * k) : FB_OK;
   if (!dy || !weights || !place || (dweights && slots && !ys)) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (dys == dy || dweights == weights) return fail(FB_ERR_INVALID_ARG, "%s: an output is one of the inputs it must not be", name);
-  const bool vec = cols % 4 == 0 && aligned16(dy) && (!dweights || aligned16(ys)) && (!dys || aligned16(dys));
-  const unsigned grid = grid_full(tokens);
-  if (vec) moe_combine_bwd_kernel<4><<<grid, kRowThreads, 0, stream>>>(dy, ys, weights, place, tokens, (uint32_t)k, cols, slots, dys, dweights);
-  else moe_combine_bwd_kernel<1><<<grid, kRowThreads, 0, stream>>>(dy, ys, weights, place, tokens, (uint32_t)k, cols, slots, dys, dweights);
+  const int vec = row_vec(cols, dy, dweights ? ys : dy, dys);
+  // A warp per token up to 64 vectors a row, else a CTA with a thread per vector, at most 256.
+  const uint64_t vpt = cols / vec;
+  const bool by_warp = vpt <= 64;
+  const uint32_t threads = by_warp || vpt >= kRowThreads ? kRowThreads : (uint32_t)(vpt + 31) / 32 * 32;
+  const unsigned grid = grid_full(by_warp ? (tokens + kRowThreads / 32 - 1) / (kRowThreads / 32) : tokens);
+  const uint32_t k32 = (uint32_t)k;
+#define FB_CALL(VEC, KU)                                                                                                              \
+  if (by_warp) moe_combine_bwd_kernel<VEC, KU, true><<<grid, threads, 0, stream>>>(dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights); \
+  else moe_combine_bwd_kernel<VEC, KU, false><<<grid, threads, 0, stream>>>(dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights)
+  FB_ROW_DISPATCH(vec, k, FB_CALL);
+#undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
 }

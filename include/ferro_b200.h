@@ -610,7 +610,7 @@ FB_API int fb_moe_sort(fb_stream_t stream, const int64_t* ids, uint64_t n, uint6
  *   combine_bwd    dys[place[t, j]] = weights[t, j] * dy[t] (other rows left as they were),
  *                  dweights[t, j] = dy[t] . ys[place[t, j]] (0 where it takes no part);
  *                  either may be NULL (ys may be, without dweights); dys may be ys.
- * 1 <= k <= FB_MOE_MAX_K.  No atomics: a row has one writer and sums have a fixed
+ * 1 <= k <= FB_MOE_MAX_K, cols < 2^31.  No atomics: a row has one writer and sums have a fixed
  * order.  Two assignments must not share a place.  Outputs must not alias inputs except as said. */
 FB_API int fb_moe_dispatch_fwd(fb_stream_t stream, const float* x, const int64_t* place, uint64_t tokens, uint64_t k,
                                uint64_t cols, float* xs, uint64_t slots);

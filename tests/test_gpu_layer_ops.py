@@ -275,13 +275,18 @@ def gate_logits(kind, t, e, r):
         l[::4] = -np.inf           # tokens that choose nobody
         l[1::6, 1:] = -np.inf      # one expert left
         l[2::6] = np.finfo(np.float32).min  # the lowest finite value is no mask
+    if kind == "near":
+        # neighbours that differ in their lowest bits only, below zero too
+        l = (np.float32(1.0) + r.integers(0, 200, (t, e)).astype(np.float32) * np.float32(2.0 ** -23)).astype(np.float32)
+        l[1::2] *= -1
+        l[2::5] = np.float32(-1.5) + np.round(l[2::5] * 4) / 4 + r.integers(0, 3, l[2::5].shape).astype(np.float32) * np.float32(2.0 ** -22)
     if kind == "wide":
         l *= np.float32(60)        # exponentials that vanish
     return l
 
 
 @pytest.mark.parametrize("t,e,k", GATE_SHAPES)
-@pytest.mark.parametrize("kind", ["plain", "ties", "masked", "wide"])
+@pytest.mark.parametrize("kind", ["plain", "ties", "near", "masked", "wide"])
 @pytest.mark.parametrize("renorm", [True, False])
 def test_gate_choice_weights_and_gradient(be, t, e, k, kind, renorm):
     r = np.random.default_rng(t + 31 * e + k)
@@ -308,7 +313,8 @@ def test_gate_choice_weights_and_gradient(be, t, e, k, kind, renorm):
 
 
 def test_gate_nan_and_infinity(be):
-    l = np.array([[1, np.nan, 3, np.nan], [np.inf, 2, np.inf, 1], [-np.inf, np.inf, 0, -np.inf], [0, -0.0, 0, -0.0]], np.float32)
+    minus_nan = np.uint32(0xFFC00001).view(np.float32)  # a NaN with its sign set is a NaN
+    l = np.array([[1, np.nan, 3, minus_nan], [np.inf, 2, np.inf, 1], [-np.inf, np.inf, 0, -np.inf], [0, -0.0, 0, -0.0]], np.float32)
     for renorm in (True, False):
         W, I = be.moe_gate_dev(be.alloc_from_host(l), 4, 4, 3, renorm)
         assert be.copy_i64_to_host(I).reshape(4, 3).tolist() == [[1, 3, 2], [0, 2, 1], [1, 2, -1], [0, 1, 2]]
