@@ -7,6 +7,8 @@
 // not depend on scheduling.
 #include "common.cuh"
 #include "fastdiv.cuh"
+#include "math.cuh"
+#include "reduce.cuh"
 
 namespace fb {
 
@@ -24,7 +26,7 @@ __device__ __forceinline__ float gate_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
-constexpr int kGateThreads = 256;
+constexpr int kGateThreads = 128;
 constexpr int kGateWarps = kGateThreads / 32;
 
 // Choice j of a row for lane j (-1 where there is none): k rounds of a warp-wide maximum over whole
@@ -57,103 +59,260 @@ __device__ __forceinline__ int32_t gate_choose_exact(const float* __restrict__ r
   return mine;
 }
 
-// Sorts a lane's keys, largest first (odd-even transposition: the networks are short).
-template <int NPL>
-__device__ __forceinline__ void gate_sort(uint32_t (&v)[NPL]) {
-#pragma unroll
-  for (int r = 0; r < NPL; ++r)
-#pragma unroll
-    for (int i = r & 1; i + 1 < NPL; i += 2) {
-      const uint32_t hi = max(v[i], v[i + 1]), lo = min(v[i], v[i + 1]);
-      v[i] = hi;
-      v[i + 1] = lo;
-    }
+// e^x for x <= 0: 2^(x log2 e) with the rounding of that product put back, so what is left is the
+// instruction's 2^-22 whatever x is.  Results below 2^-126 are 0.  NaN stays NaN.
+__device__ __forceinline__ float gate_exp(float x) {
+  x = fmax_nan(x, -200.0f);  // -inf would turn the correction into a NaN
+  const float t = x * 1.4426950408889634f;
+  float r = fmaf(x, 1.4426950408889634f, -t);
+  r = fmaf(x, 1.925963033500e-8f, r);  // log2 e - its f32 value
+  const float e = ex2_approx_ftz(t);
+  return fmaf(e, r * 0.6931471805599453f, e);
 }
 
-// The same through packed words: the expert's number, complemented, takes the place of the key's lowest
-// IDBITS bits, so that one warp-wide maximum gives value, index and tie-break at once and a lane
-// recognises its own entry by equality.  The order found is exact unless entries that differ only in
-// the bits cut off were met: `ok` is false then, and the caller chooses again with whole keys.  That is
-// the case if two neighbours among the chosen agree in the kept bits but not in value, or if the
-// last chosen and the first left out agree in the kept bits.
-template <int NPL>
-__device__ __forceinline__ int32_t gate_choose_packed(const float* __restrict__ row, const float (&v)[NPL], uint32_t experts,
-                                                      uint32_t k, int lane, float& value, bool& ok) {
-  constexpr uint32_t kIds = 32 * NPL;  // a power of two
-  uint32_t w[NPL];
+// ---- lists in registers, largest first
+__device__ __forceinline__ void gate_order(uint32_t& a, uint32_t& b) {
+  const uint32_t hi = max(a, b), lo = min(a, b);
+  a = hi;
+  b = lo;
+}
+// Batcher's odd-even merge sort of v[LO .. LO + N) (19 exchanges for 8), as compile-time recursion.
+template <int N, int LO, int R, int M>
+__device__ __forceinline__ void gate_sort_merge(uint32_t (&v)[M]) {
+  if constexpr (2 * R < N) {
+    gate_sort_merge<N, LO, 2 * R>(v);
+    gate_sort_merge<N, LO + R, 2 * R>(v);
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) {
-    const uint32_t e = i * 32 + lane;
-    w[i] = e < experts ? (gate_key(v[i]) & ~(kIds - 1)) | (kIds - 1 - e) : 0u;
+    for (int i = LO + R; i + R < LO + N; i += 2 * R) gate_order(v[i], v[i + R]);
+  } else {
+    gate_order(v[LO], v[LO + R]);
   }
-  if constexpr (NPL <= 8) gate_sort(w);
-  uint32_t mine = 0, next = 0;  // next: the first left out
-  for (uint32_t j = 0; j <= k; ++j) {
-    uint32_t head = w[0];
-    if constexpr (NPL > 8) {
+}
+template <int N, int LO, int M>
+__device__ __forceinline__ void gate_sort(uint32_t (&v)[M]) {
+  if constexpr (N > 1) {
+    gate_sort<N / 2, LO>(v);
+    gate_sort<N / 2, LO + N / 2>(v);
+    gate_sort_merge<N, LO, 1>(v);
+  }
+}
+// a = the N largest of two sorted lists, sorted: the larger of a_i and b_(N-1-i) are those N and form a
+// bitonic sequence.
+template <int N>
+__device__ __forceinline__ void gate_merge(uint32_t (&a)[N], const uint32_t (&b)[N]) {
 #pragma unroll
-      for (int i = 1; i < NPL; ++i) head = max(head, w[i]);
-    }
-    const uint32_t win = __reduce_max_sync(0xffffffffu, head);
-    if (j == k) {
-      next = win;
-      break;
-    }
-    if ((uint32_t)lane == j) mine = win;
-    if constexpr (NPL <= 8) {
-      if (head == win) {
+  for (int i = 0; i < N; ++i) a[i] = max(a[i], b[N - 1 - i]);
 #pragma unroll
-        for (int i = 0; i + 1 < NPL; ++i) w[i] = w[i + 1];
-        w[NPL - 1] = 0;
-      }
+  for (int s = N / 2; s >= 1; s /= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & s) == 0) gate_order(a[i], a[i + s]);
+}
+// The N largest of v, sorted; the lists of N are sorted and merged one after the other.
+template <int N, int LO, int M>
+__device__ __forceinline__ void gate_top(uint32_t (&v)[M], uint32_t (&top)[N]) {
+  if constexpr (LO < M) {
+    gate_sort<N, LO>(v);
+    uint32_t b[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = v[LO + i];
+    if constexpr (LO == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) top[i] = b[i];
     } else {
-#pragma unroll
-      for (int i = 0; i < NPL; ++i) w[i] = w[i] == win ? 0u : w[i];
+      gate_merge<N>(top, b);
     }
+    gate_top<N, LO + N>(v, top);
   }
-  const bool real = mine > kGateMasked;  // lanes from k on hold 0
-  const int32_t id = real ? (int32_t)(kIds - 1 - (mine & (kIds - 1))) : -1;
-  value = real ? __ldg(row + id) + 0.0f : 0.0f;
-  const uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
-  const float after_value = __shfl_down_sync(0xffffffffu, value, 1);
-  bool clash = false;
-  if (real && (uint32_t)lane + 1 < k) clash = (mine & ~(kIds - 1)) == (after & ~(kIds - 1)) && value != after_value && !(value != value && after_value != after_value);
-  if (real && (uint32_t)lane + 1 == k) clash = (mine & ~(kIds - 1)) == (next & ~(kIds - 1));
-  ok = !__any_sync(0xffffffffu, clash);
-  return id;
 }
 
-template <int NPL, bool RENORM>
-__global__ void __launch_bounds__(kGateThreads)
-moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t experts, uint32_t k,
+// L lanes of a warp hold a token's row, V values each.  Where the row is read in vectors of 4, register
+// r of lane l is expert (r / 4) * 4 L + 4 l + r % 4, else r L + l.
+template <int L, int V>
+__device__ __forceinline__ uint32_t gate_expert(int r, int l, bool vec) {
+  return V % 4 == 0 && vec ? (r / 4) * (4 * L) + 4 * l + r % 4 : r * L + l;
+}
+template <int L, int V>
+__device__ __forceinline__ void gate_load(const float* __restrict__ row, uint32_t experts, int l, bool vec, bool live, float (&v)[V]) {
+  if (V % 4 == 0 && vec) {
+#pragma unroll
+    for (int r = 0; r < V; r += 4) {
+      const uint32_t e = gate_expert<L, V>(r, l, true);
+      const float4 t = live && e < experts ? __ldg(reinterpret_cast<const float4*>(row + e)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      v[r] = t.x;
+      if constexpr (V % 4 == 0) { v[r + 1] = t.y; v[r + 2] = t.z; v[r + 3] = t.w; }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < V; ++r) {
+      const uint32_t e = r * L + l;
+      v[r] = live && e < experts ? __ldg(row + e) : -INFINITY;
+    }
+  }
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Choice through packed words: the expert's number, complemented, takes the place of the key's lowest
+// bits, so that integer maxima order value, then index (ties: lowest first), and carry the index along.
+// A lane sorts its values' KL largest, lists are merged across the token's L lanes by shuffles; two
+// instructions an exchange instead of the five that separate keys and indices would take.
+//
+// The order found is exact unless entries that differ only in the bits cut off were met: two neighbours
+// among the chosen that agree in the kept bits but not in value, or one left out that agrees in the
+// kept bits with the last chosen.  Such a token is chosen again on whole keys by the whole warp.
+//
+// Bound by the integer pipe, which issues half the rate of the others: per token of 128 experts and 8
+// choices about 100 instructions, 12 us for 32768 tokens; one warp-wide maximum per choice took 407 (16 us).
+template <int KL, int L, int V>
+__global__ void __launch_bounds__(kGateThreads, V <= 16 ? 8 : 4)
+moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t experts, uint32_t k, bool renorm, bool vec,
                     float* __restrict__ weights, int64_t* __restrict__ ids) {
+  static_assert(KL <= L, "lane l of a token reports choice l");
+  constexpr uint32_t kIds = L * V, kKept = ~(kIds - 1);  // a power of two
+  constexpr int kTokens = 32 / L;                        // per warp
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, g = lane / L;
+  const uint64_t step = (uint64_t)gridDim.x * kGateWarps * kTokens;
+  for (uint64_t t0 = ((uint64_t)blockIdx.x * kGateWarps + warp) * kTokens; t0 < tokens; t0 += step) {
+    const uint64_t t = t0 + g;
+    const bool live = t < tokens;
+    const float* row = logits + t * experts;
+    float v[V];
+    gate_load<L, V>(row, experts, l, vec, live, v);
+    uint32_t w[V], top[KL];
+#pragma unroll
+    for (int r = 0; r < V; ++r) w[r] = (gate_key(v[r]) & kKept) | (kIds - 1 - gate_expert<L, V>(r, l, vec));
+    {
+      uint32_t c[V < KL ? KL : V];
+#pragma unroll
+      for (int r = 0; r < (V < KL ? KL : V); ++r) c[r] = r < V ? w[r] : 0u;
+      gate_top<KL, 0>(c, top);
+    }
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) {
+      uint32_t b[KL];
+#pragma unroll
+      for (int i = 0; i < KL; ++i) b[i] = __shfl_xor_sync(0xffffffffu, top[i], o);
+      gate_merge<KL>(top, b);
+    }
+    // lane l: choice l, the one behind it and the last
+    uint32_t mine = 0, after = 0, last = 0;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      if (i == l) mine = top[i];
+      if (i == l + 1) after = top[i];
+      if (i + 1 == (int)k) last = top[i];
+    }
+    const bool mine_in = l < (int)k && mine > kGateMasked;
+    int32_t id = mine_in ? (int32_t)(kIds - 1 - (mine & (kIds - 1))) : -1;
+    float value = mine_in ? __ldg(row + id) : 0.0f;
+    const float after_value = __shfl_down_sync(0xffffffffu, value, 1);
+    bool clash = false;
+    if (mine_in && l + 1 < (int)k && after > kGateMasked)
+      clash = ((mine ^ after) & kKept) == 0 && __float_as_uint(value + 0.0f) != __float_as_uint(after_value + 0.0f);
+    // How many get as far as the last chosen in the kept bits: k, or too many.  Counted for every token,
+    // with or without a last: all lanes of the warp have to meet in the shuffles.
+    uint32_t reach = 0;
+#pragma unroll
+    for (int r = 0; r < V; ++r) reach += w[r] >= (last & kKept);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) reach += __shfl_xor_sync(0xffffffffu, reach, o);
+    clash |= last > kGateMasked && reach > k;
+    const uint32_t groups = L == 32 ? 0xffffffffu : ((1u << (L & 31)) - 1u);
+    uint32_t again = __ballot_sync(0xffffffffu, clash);
+    while (again) {  // rare; every lane works on the token of the lowest lane that asks
+      const int who = (__ffs(again) - 1) / L;
+      again &= ~(groups << (who * L));
+      const int32_t found = gate_choose_exact<L * V / 32>(logits + (t0 + who) * experts, experts, k, lane);
+      const int32_t theirs = __shfl_sync(0xffffffffu, found, l);
+      if (g == who) {
+        id = l < (int)k ? theirs : -1;
+        value = id >= 0 ? __ldg(row + id) : 0.0f;
+      }
+    }
+    const float m = __shfl_sync(0xffffffffu, value, g * L);  // the largest, where there is one
+    const float mass = id >= 0 ? gate_exp(value - m) : 0.0f;
+    float total;
+    if (renorm) {
+      total = lanes_sum<L>(mass);
+    } else {
+      total = 0.0f;
+#pragma unroll
+      for (int r = 0; r < V; ++r) total += gate_exp(v[r] - m);
+      total = lanes_sum<L>(total);
+    }
+    if (live && l < (int)k) {
+      weights[t * k + l] = id >= 0 ? mass / total : 0.0f;
+      ids[t * k + l] = id;
+    }
+  }
+}
+
+// More than 8 choices: a warp per token, k warp-wide maxima over the lanes' largest packed words, one
+// more for the first left out.  A lane keeps its words sorted and moves them up when its head is taken
+// (up to 8 a lane), or strikes the taken one out.  Lists of 16 merged as above would take 24.7 to 30.5 us
+// for 32768 tokens, 10 choices of 32 to 128 experts.
+template <int NPL>
+__global__ void __launch_bounds__(kGateThreads)
+moe_gate_fwd_many_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t experts, uint32_t k, bool renorm,
+                         float* __restrict__ weights, int64_t* __restrict__ ids) {
+  constexpr uint32_t kIds = 32 * NPL, kKept = ~(kIds - 1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (uint64_t t = (uint64_t)blockIdx.x * kGateWarps + warp; t < tokens; t += (uint64_t)gridDim.x * kGateWarps) {
     const float* row = logits + t * experts;
     float v[NPL];
+    gate_load<32, NPL>(row, experts, lane, false, true, v);
+    uint32_t w[NPL];
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      const uint32_t e = i * 32 + lane;
-      v[i] = e < experts ? __ldg(row + e) : -INFINITY;
+    for (int r = 0; r < NPL; ++r) w[r] = (gate_key(v[r]) & kKept) | (kIds - 1 - (r * 32 + lane));
+    if constexpr (NPL <= 8) gate_sort<NPL, 0>(w);
+    uint32_t mine = 0, next = 0;  // next: the first left out
+    for (uint32_t j = 0;; ++j) {
+      uint32_t head = w[0];
+      if constexpr (NPL > 8) {
+#pragma unroll
+        for (int r = 1; r < NPL; ++r) head = max(head, w[r]);
+      }
+      const uint32_t win = __reduce_max_sync(0xffffffffu, head);
+      if (j == k) {
+        next = win;
+        break;
+      }
+      mine = (uint32_t)lane == j ? win : mine;
+      if constexpr (NPL <= 8) {
+        const bool hit = head == win;
+#pragma unroll
+        for (int r = 0; r < NPL; ++r) w[r] = hit ? (r + 1 < NPL ? w[r + 1] : 0u) : w[r];
+      } else {
+#pragma unroll
+        for (int r = 0; r < NPL; ++r) w[r] = w[r] == win ? 0u : w[r];
+      }
     }
-    float value;
-    bool ok;
-    int32_t id = gate_choose_packed<NPL>(row, v, experts, k, lane, value, ok);
-    if (!ok) {
+    const bool in = mine > kGateMasked;  // lanes from k on hold 0
+    int32_t id = in ? (int32_t)(kIds - 1 - (mine & (kIds - 1))) : -1;
+    float value = in ? __ldg(row + id) : 0.0f;
+    uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
+    const float after_value = __shfl_down_sync(0xffffffffu, value, 1);
+    bool clash = in && (uint32_t)lane + 1 < k && after > kGateMasked && ((mine ^ after) & kKept) == 0 &&
+                 __float_as_uint(value + 0.0f) != __float_as_uint(after_value + 0.0f);
+    clash |= in && (uint32_t)lane + 1 == k && next > kGateMasked && ((mine ^ next) & kKept) == 0;
+    if (__any_sync(0xffffffffu, clash)) {
       id = gate_choose_exact<NPL>(row, experts, k, lane);
       value = id >= 0 ? __ldg(row + id) : 0.0f;
     }
-    const float m = __shfl_sync(0xffffffffu, value, 0);  // the largest, where there is one
-    const float mass = id >= 0 ? expf(value - m) : 0.0f;
-    float total;
-    if (RENORM) {
-      total = warp_sum(mass);
-    } else {
+    const float m = __shfl_sync(0xffffffffu, value, 0);
+    const float mass = id >= 0 ? gate_exp(value - m) : 0.0f;
+    float total = mass;
+    if (!renorm) {
       total = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) total += v[i] == -INFINITY ? 0.0f : expf(v[i] - m);
-      total = warp_sum(total);
+      for (int r = 0; r < NPL; ++r) total += gate_exp(v[r] - m);
     }
+    total = warp_sum(total);
     if ((uint32_t)lane < k) {
       weights[t * k + lane] = id >= 0 ? mass / total : 0.0f;
       ids[t * k + lane] = id;
@@ -161,62 +320,91 @@ moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t 
   }
 }
 
-// Lane j takes choice j; the row is laid out in shared memory, the chosen entries written over it.  A
-// chosen entry is w_j (dw_j - sum w dw) in both forms: the saved weight is its probability.
-template <int NPL, bool RENORM>
+// L lanes per token; lane l takes choices l, l + L, ...  The row is laid out in shared memory and the
+// chosen entries written over it.  A chosen entry is w_j (dw_j - sum w dw) in both forms: the saved
+// weight is its probability.
+template <int L, int V>
 __global__ void __launch_bounds__(kGateThreads)
 moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict__ logits, const float* __restrict__ weights,
-                    const int64_t* __restrict__ ids, uint64_t tokens, uint32_t experts, uint32_t k,
+                    const int64_t* __restrict__ ids, uint64_t tokens, uint32_t experts, uint32_t k, bool renorm, bool vec,
                     float* __restrict__ dlogits) {
-  __shared__ float rows[kGateWarps][32 * NPL];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* out = rows[warp];
-  for (uint64_t t = (uint64_t)blockIdx.x * kGateWarps + warp; t < tokens; t += (uint64_t)gridDim.x * kGateWarps) {
-    float w = 0.0f, dw = 0.0f;
-    int64_t id = -1;
-    if ((uint32_t)lane < k) {
-      id = __ldg(ids + t * k + lane);
-      if (id < 0 || id >= (int64_t)experts) id = -1;
-      else {
-        w = __ldg(weights + t * k + lane);
-        dw = __ldg(dweights + t * k + lane);
+  constexpr int kTokens = 32 / L, kMine = FB_MOE_MAX_K / L;
+  __shared__ __align__(16) float rows[kGateThreads / L][L * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, g = lane / L;
+  float* out = rows[warp * kTokens + g];
+  const uint64_t step = (uint64_t)gridDim.x * kGateWarps * kTokens;
+  for (uint64_t t0 = ((uint64_t)blockIdx.x * kGateWarps + warp) * kTokens; t0 < tokens; t0 += step) {
+    const uint64_t t = t0 + g;
+    const bool live = t < tokens;
+    float v[V];
+    if (!renorm) gate_load<L, V>(logits + t * experts, experts, l, vec, live, v);
+    float w[kMine], dw[kMine], dot = 0.0f;
+    int32_t id[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const uint32_t j = i * L + l;
+      id[i] = -1;
+      w[i] = dw[i] = 0.0f;
+      if (live && j < k) {
+        const int64_t e = __ldg(ids + t * k + j);
+        if (e >= 0 && e < (int64_t)experts) {
+          id[i] = (int32_t)e;
+          w[i] = __ldg(weights + t * k + j);
+          dw[i] = __ldg(dweights + t * k + j);
+          dot = fmaf(w[i], dw[i], dot);
+        }
       }
     }
-    float p[NPL];
-    if (!RENORM) {
+    dot = lanes_sum<L>(dot);
+    if (renorm) {
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) {
-        const uint32_t e = i * 32 + lane;
-        p[i] = e < experts ? __ldg(logits + t * experts + e) : -INFINITY;
-      }
-    }
-    const float dot = warp_sum(w * dw);
-    if (!RENORM) {
-      uint32_t best = gate_key(p[0]);
+      for (int r = 0; r < V; ++r) v[r] = 0.0f;
+    } else {
+      float m = v[0];
 #pragma unroll
-      for (int i = 1; i < NPL; ++i) best = max(best, gate_key(p[i]));
-      const float m = gate_value(__reduce_max_sync(0xffffffffu, best));
+      for (int r = 1; r < V; ++r) m = fmax_nan(m, v[r]);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      // a row of nothing but masked entries: every exponent NaN, every entry 0 below
       float total = 0.0f;
+      uint32_t masked = 0;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) {
-        p[i] = p[i] == -INFINITY ? -0.0f : expf(p[i] - m);  // -0: masked, stays 0 whatever total is
-        total += p[i];
+      for (int r = 0; r < V; ++r) {
+        if (v[r] == -INFINITY) masked |= 1u << r;
+        v[r] = v[r] == -INFINITY ? 0.0f : gate_exp(v[r] - m);
+        total += v[r];
       }
-      total = warp_sum(total);
+      total = lanes_sum<L>(total);
       const float f = -dot / total;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) out[i * 32 + lane] = __float_as_uint(p[i]) == 0x80000000u ? 0.0f : p[i] * f;
+      for (int r = 0; r < V; ++r) v[r] = (masked >> r) & 1 ? 0.0f : v[r] * f;
+    }
+    if (V % 4 == 0 && vec) {
+#pragma unroll
+      for (int r = 0; r < V; r += 4)
+        if constexpr (V % 4 == 0) *reinterpret_cast<float4*>(out + gate_expert<L, V>(r, l, true)) = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
     } else {
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) out[i * 32 + lane] = 0.0f;
+      for (int r = 0; r < V; ++r) out[r * L + l] = v[r];
     }
     __syncwarp();
-    if (id >= 0) out[id] = w * (dw - dot);
-    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      const uint32_t e = i * 32 + lane;
-      if (e < experts) dlogits[t * experts + e] = out[e];
+    for (int i = 0; i < kMine; ++i)
+      if (id[i] >= 0) out[id[i]] = w[i] * (dw[i] - dot);
+    __syncwarp();
+    if (live) {
+      float* to = dlogits + t * experts;
+      if (V % 4 == 0 && vec) {
+#pragma unroll
+        for (int r = 0; r < V; r += 4) {
+          const uint32_t e = gate_expert<L, V>(r, l, true);
+          if (e < experts) *reinterpret_cast<float4*>(to + e) = *reinterpret_cast<const float4*>(out + e);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < V; ++r)
+          if (r * L + l < experts) to[r * L + l] = out[r * L + l];
+      }
     }
     __syncwarp();
   }
@@ -421,24 +609,38 @@ struct RowVec {
   }
 };
 
-// Where a thread stands: a token's row is cut into vectors, a CTA takes `tpb` whole tokens or one of
-// `bpt` pieces of a token, a thread one vector.
+// Where a thread stands.  A token's row is cut into vectors.  Narrow rows: a CTA takes `tpb` tokens, a
+// thread one vector.  Wider ones: a CTA takes a token, a thread every blockDim.x-th vector; where that
+// gives too few CTAs, one of `bpt` pieces of a token.  With 8192 tokens, 8 choices and 2048 columns the
+// gather runs at 102 % of the copy rate with a CTA per token and at 80 % with two CTAs per token, whose
+// halves of a row reach DRAM at different times.
 struct RowMap {
   uint64_t tokens, cols, slots, blocks;
   uint32_t k, vpt;    // vectors per row
   uint32_t tpb, bpt;
+  uint32_t piece;     // vectors per piece (bpt > 1)
   FastDiv d_vpt;
 };
-__device__ __forceinline__ bool row_place(const RowMap& M, uint64_t blk, uint64_t& t, uint32_t& vec) {
-  if (M.bpt == 1) {
+// First vector of this thread, one behind its last, and their step; false: nothing to do.
+__device__ __forceinline__ bool row_place(const RowMap& M, uint64_t blk, uint64_t& t, uint32_t& vec, uint32_t& end) {
+  if (M.tpb > 1) {
     const uint32_t tl = fdiv(threadIdx.x, M.d_vpt);
     vec = threadIdx.x - tl * M.vpt;
+    end = vec + 1;
     t = blk * M.tpb + tl;
     return tl < M.tpb && t < M.tokens;
   }
-  t = blk / M.bpt;
-  vec = (uint32_t)(blk - t * M.bpt) * kRowThreads + threadIdx.x;
-  return vec < M.vpt;
+  if (M.bpt == 1) {
+    t = blk;
+    vec = threadIdx.x;
+    end = M.vpt;
+  } else {
+    t = blk / M.bpt;
+    const uint32_t lo = (uint32_t)(blk - t * M.bpt) * M.piece;
+    vec = lo + threadIdx.x;
+    end = min(lo + M.piece, M.vpt);
+  }
+  return true;
 }
 
 __device__ __forceinline__ int64_t slot_of(const int64_t* place, uint64_t a, uint64_t slots) {
@@ -448,60 +650,65 @@ __device__ __forceinline__ int64_t slot_of(const int64_t* place, uint64_t a, uin
 
 // xs[place[t, j]] = x[t], KU choices at a time: their places are loaded before the first store.
 template <int VEC, int KU>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, KU == 8 ? 4 : 5)
 moe_scatter_kernel(const float* __restrict__ x, const int64_t* __restrict__ place, const __grid_constant__ RowMap M,
                    float* __restrict__ xs) {
   for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
     uint64_t t;
-    uint32_t vec;
-    if (!row_place(M, blk, t, vec)) continue;
-    const uint64_t c = (uint64_t)vec * VEC;
-    RowVec<VEC> v;
-    v.load(x + t * M.cols + c);
-    for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
-      int64_t s[KU];
+    uint32_t vec, end;
+    if (!row_place(M, blk, t, vec, end)) continue;
+    for (; vec < end; vec += blockDim.x) {
+      const uint64_t c = (uint64_t)vec * VEC;
+      RowVec<VEC> v;
+      v.load(x + t * M.cols + c);
+      for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
+        int64_t s[KU];
 #pragma unroll
-      for (int j = 0; j < KU; ++j) s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
+        for (int j = 0; j < KU; ++j) s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
 #pragma unroll
-      for (int j = 0; j < KU; ++j)
-        if (s[j] >= 0) v.store(xs + (uint64_t)s[j] * M.cols + c);
+        for (int j = 0; j < KU; ++j)
+          if (s[j] >= 0) v.store(xs + (uint64_t)s[j] * M.cols + c);
+      }
     }
   }
 }
 
 // y[t] = sum over j of (weights[t, j] *) ys[place[t, j]], KU rows in flight, added in the order of j.
+// Bound by HBM; what counts is enough CTAs per SM (five with KU 4) to cover the load of the places.
 template <int VEC, int KU, bool WEIGHTED>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, KU == 8 ? 3 : 5)
 moe_gather_kernel(const float* __restrict__ ys, const float* __restrict__ weights, const int64_t* __restrict__ place,
                   const __grid_constant__ RowMap M, float* __restrict__ y) {
   for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
     uint64_t t;
-    uint32_t vec;
-    if (!row_place(M, blk, t, vec)) continue;
-    const uint64_t c = (uint64_t)vec * VEC;
-    RowVec<VEC> acc;
+    uint32_t vec, end;
+    if (!row_place(M, blk, t, vec, end)) continue;
+    for (; vec < end; vec += blockDim.x) {
+      const uint64_t c = (uint64_t)vec * VEC;
+      RowVec<VEC> acc;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc.v[i] = 0.0f;
-    for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
-      int64_t s[KU];
-      float w[KU];
+      for (int i = 0; i < VEC; ++i) acc.v[i] = 0.0f;
+      for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
+        int64_t s[KU];
+        float w[KU];
 #pragma unroll
-      for (int j = 0; j < KU; ++j) {
-        s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
-        if (WEIGHTED) w[j] = j0 + j < M.k ? __ldg(weights + t * M.k + j0 + j) : 0.0f;
-      }
-      RowVec<VEC> r[KU];
-#pragma unroll
-      for (int j = 0; j < KU; ++j)
-        if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * M.cols + c);
-#pragma unroll
-      for (int j = 0; j < KU; ++j)
-        if (s[j] >= 0) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) acc.v[i] = WEIGHTED ? fmaf(r[j].v[i], w[j], acc.v[i]) : acc.v[i] + r[j].v[i];
+        for (int j = 0; j < KU; ++j) {
+          s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
+          if (WEIGHTED) w[j] = j0 + j < M.k ? __ldg(weights + t * M.k + j0 + j) : 0.0f;
         }
+        RowVec<VEC> r[KU];
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+          if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * M.cols + c);
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+          if (s[j] >= 0) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc.v[i] = WEIGHTED ? fmaf(r[j].v[i], w[j], acc.v[i]) : acc.v[i] + r[j].v[i];
+          }
+      }
+      acc.store(y + t * M.cols + c);
     }
-    acc.store(y + t * M.cols + c);
   }
 }
 
@@ -591,17 +798,31 @@ static int rows_check(const char* name, uint64_t tokens, uint64_t k, uint64_t co
   return FB_OK;
 }
 
-static RowMap row_map(uint64_t tokens, uint64_t k, uint64_t cols, uint64_t slots, int vec) {
+// Fewer CTAs than the SMs hold when each takes a token: rows are cut into pieces and all choices of a
+// token taken at once, for the shortest chain of loads instead of the best stream.
+static bool few_tokens(uint64_t tokens) { return tokens < (uint64_t)device_info().sm_count * 4; }
+
+static RowMap row_map(uint64_t tokens, uint64_t k, uint64_t cols, uint64_t slots, int vec, uint32_t* threads) {
   RowMap m = {};
   m.tokens = tokens;
   m.cols = cols;
   m.slots = slots;
   m.k = (uint32_t)k;
   m.vpt = (uint32_t)(cols / vec);
-  m.tpb = m.vpt < kRowThreads ? kRowThreads / m.vpt : 1;
-  m.bpt = (m.vpt + kRowThreads - 1) / kRowThreads;
+  m.tpb = m.vpt <= kRowThreads / 2 ? kRowThreads / m.vpt : 1;
+  m.bpt = 1;
   m.d_vpt = make_fastdiv(m.vpt);
-  m.blocks = (tokens + m.tpb - 1) / m.tpb * m.bpt;
+  *threads = kRowThreads;
+  if (m.tpb == 1) {
+    // equal shares: as many threads as divide the row into the least number of rounds
+    const uint32_t rounds = (m.vpt + kRowThreads - 1) / kRowThreads;
+    *threads = ((m.vpt + rounds - 1) / rounds + 31) / 32 * 32;
+    if (rounds > 1 && few_tokens(tokens)) {
+      m.piece = *threads;
+      m.bpt = (m.vpt + m.piece - 1) / m.piece;
+    }
+  }
+  m.blocks = m.tpb > 1 ? (tokens + m.tpb - 1) / m.tpb : tokens * m.bpt;
   return m;
 }
 
@@ -612,15 +833,29 @@ static int row_vec(uint64_t cols, const void* a, const void* b, const void* c = 
 }
 
 // CALL(VEC, KU) for the access width and the number of choices taken at a time.
-#define FB_ROW_DISPATCH(vec, k, CALL)                             \
-  do {                                                            \
-    if ((vec) == 4) { if ((k) <= 2) { CALL(4, 2); } else if ((k) <= 4) { CALL(4, 4); } else { CALL(4, 8); } } \
-    else if ((vec) == 2) { if ((k) <= 2) { CALL(2, 2); } else if ((k) <= 4) { CALL(2, 4); } else { CALL(2, 8); } } \
-    else { if ((k) <= 2) { CALL(1, 2); } else if ((k) <= 4) { CALL(1, 4); } else { CALL(1, 8); } } \
+#define FB_ROW_KU(VEC, k, wide, CALL)  \
+  if ((k) <= 2) { CALL(VEC, 2); }      \
+  else if ((k) <= 4 || !(wide)) { CALL(VEC, 4); } \
+  else { CALL(VEC, 8); }
+#define FB_ROW_DISPATCH(vec, k, wide, CALL)               \
+  do {                                                    \
+    if ((vec) == 4) { FB_ROW_KU(4, k, wide, CALL) }       \
+    else if ((vec) == 2) { FB_ROW_KU(2, k, wide, CALL) }  \
+    else { FB_ROW_KU(1, k, wide, CALL) }                  \
   } while (0)
 
-// CALL(NPL) for the number of experts a lane holds.
-#define FB_GATE_DISPATCH(experts, CALL)            \
+// CALL(L, V): lanes per token and values per lane that hold the experts of a row.
+#define FB_GATE_ROWS(experts, CALL)                                              \
+  do {                                                                           \
+    if ((experts) <= 32) { CALL(8, 4); }                           \
+    else if ((experts) <= 64) { CALL(8, 8); }                      \
+    else if ((experts) <= 128) { CALL(8, 16); }                    \
+    else if ((experts) <= 256) { CALL(16, 16); }                                 \
+    else if ((experts) <= 512) { CALL(32, 16); }                                 \
+    else { CALL(32, 32); }                                                       \
+  } while (0)
+// CALL(NPL): experts per lane of a whole warp.
+#define FB_GATE_WARP(experts, CALL)                \
   do {                                             \
     if ((experts) <= 32) { CALL(1); }              \
     else if ((experts) <= 64) { CALL(2); }         \
@@ -644,12 +879,23 @@ int fb_moe_gate_fwd(fb_stream_t stream, const float* logits, uint64_t tokens, ui
   if (int rc = gate_check(name, tokens, experts, k)) return rc;
   if (tokens == 0) return FB_OK;
   if (!logits || !weights || !ids) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
-  const unsigned grid = grid_full((tokens + kGateThreads / 32 - 1) / (kGateThreads / 32));
-#define FB_CALL(NPL)                                                                                                          \
-  if (renorm) moe_gate_fwd_kernel<NPL, true><<<grid, kGateThreads, 0, stream>>>(logits, tokens, (uint32_t)experts, (uint32_t)k, weights, ids); \
-  else moe_gate_fwd_kernel<NPL, false><<<grid, kGateThreads, 0, stream>>>(logits, tokens, (uint32_t)experts, (uint32_t)k, weights, ids)
-  FB_GATE_DISPATCH(experts, FB_CALL);
+  const bool vec = experts % 4 == 0 && aligned16(logits);
+  const uint32_t E = (uint32_t)experts, K = (uint32_t)k;
+#define FB_CALL(KL, L, V)                                                                                        \
+  moe_gate_fwd_kernel<KL, L, V><<<grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L)), kGateThreads, 0, stream>>>( \
+      logits, tokens, E, K, renorm != 0, vec, weights, ids)
+#define FB_CALL2(L, V) FB_CALL(2, L, V)
+#define FB_CALL8(L, V) FB_CALL(8, L, V)
+#define FB_MANY(NPL)                                                                                             \
+  moe_gate_fwd_many_kernel<NPL><<<grid_full((tokens + kGateWarps - 1) / kGateWarps), kGateThreads, 0, stream>>>( \
+      logits, tokens, E, K, renorm != 0, weights, ids)
+  if (k <= 2) FB_GATE_ROWS(experts, FB_CALL2);
+  else if (k <= 8) FB_GATE_ROWS(experts, FB_CALL8);
+  else FB_GATE_WARP(experts, FB_MANY);
 #undef FB_CALL
+#undef FB_CALL2
+#undef FB_CALL8
+#undef FB_MANY
   FB_LAUNCHED(name);
   return FB_OK;
 }
@@ -660,11 +906,11 @@ int fb_moe_gate_bwd(fb_stream_t stream, const float* dweights, const float* logi
   if (int rc = gate_check(name, tokens, experts, k)) return rc;
   if (tokens == 0) return FB_OK;
   if (!dweights || !weights || !ids || !dlogits || (!renorm && !logits)) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
-  const unsigned grid = grid_full((tokens + kGateThreads / 32 - 1) / (kGateThreads / 32));
-#define FB_CALL(NPL)                                                                                                          \
-  if (renorm) moe_gate_bwd_kernel<NPL, true><<<grid, kGateThreads, 0, stream>>>(dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, dlogits); \
-  else moe_gate_bwd_kernel<NPL, false><<<grid, kGateThreads, 0, stream>>>(dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, dlogits)
-  FB_GATE_DISPATCH(experts, FB_CALL);
+  const bool vec = experts % 4 == 0 && aligned16(dlogits) && (renorm || aligned16(logits));
+#define FB_CALL(L, V)                                                                                            \
+  moe_gate_bwd_kernel<L, V><<<grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L)), kGateThreads, 0, stream>>>( \
+      dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, renorm != 0, vec, dlogits)
+  FB_GATE_ROWS(experts, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
@@ -722,10 +968,11 @@ int fb_moe_dispatch_fwd(fb_stream_t stream, const float* x, const int64_t* place
   if (!x || !place || !xs) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (xs == x) return fail(FB_ERR_INVALID_ARG, "%s: xs must not be x", name);
   const int vec = row_vec(cols, x, xs);
-  const RowMap m = row_map(tokens, k, cols, slots, vec);
+  uint32_t threads;
+  const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
   const unsigned grid = grid_full(m.blocks);
-#define FB_CALL(VEC, KU) moe_scatter_kernel<VEC, KU><<<grid, kRowThreads, 0, stream>>>(x, place, m, xs)
-  FB_ROW_DISPATCH(vec, k, FB_CALL);
+#define FB_CALL(VEC, KU) moe_scatter_kernel<VEC, KU><<<grid, threads, 0, stream>>>(x, place, m, xs)
+  FB_ROW_DISPATCH(vec, k, true, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
@@ -738,12 +985,13 @@ static int gather_rows(cudaStream_t stream, const char* name, const float* ys, c
   if ((slots && !ys) || !place || !y) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (ys == y) return fail(FB_ERR_INVALID_ARG, "%s: the output must not be the input", name);
   const int vec = row_vec(cols, ys, y);
-  const RowMap m = row_map(tokens, k, cols, slots, vec);
+  uint32_t threads;
+  const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
   const unsigned grid = grid_full(m.blocks);
 #define FB_CALL(VEC, KU)                                                                                            \
-  if (weights) moe_gather_kernel<VEC, KU, true><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, m, y);        \
-  else moe_gather_kernel<VEC, KU, false><<<grid, kRowThreads, 0, stream>>>(ys, weights, place, m, y)
-  FB_ROW_DISPATCH(vec, k, FB_CALL);
+  if (weights) moe_gather_kernel<VEC, KU, true><<<grid, threads, 0, stream>>>(ys, weights, place, m, y);            \
+  else moe_gather_kernel<VEC, KU, false><<<grid, threads, 0, stream>>>(ys, weights, place, m, y)
+  FB_ROW_DISPATCH(vec, k, few_tokens(tokens), FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
@@ -778,7 +1026,7 @@ int fb_moe_combine_bwd(fb_stream_t stream, const float* dy, const float* ys, con
 #define FB_CALL(VEC, KU)                                                                                                              \
   if (by_warp) moe_combine_bwd_kernel<VEC, KU, true><<<grid, threads, 0, stream>>>(dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights); \
   else moe_combine_bwd_kernel<VEC, KU, false><<<grid, threads, 0, stream>>>(dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights)
-  FB_ROW_DISPATCH(vec, k, FB_CALL);
+  FB_ROW_DISPATCH(vec, k, true, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
