@@ -14,7 +14,6 @@
 #include "common.cuh"
 #include "fastdiv.cuh"
 #include "philox.cuh"
-#include "reduce.cuh"
 
 namespace fb {
 
@@ -99,32 +98,163 @@ dropout_kernel(const float* x, const float* __restrict__ bias, const float* resi
   }
 }
 
-// Column-sum source of the bias gradient: the masked gradient, stored to dx on the way.
-struct DropBwdSrc {
-  const float* g;
-  float* dx;
-  uint64_t cols;
-  DropMask M;
-  template <int VEC>
-  __device__ __forceinline__ void load(uint64_t, uint64_t r, uint64_t c, float (&v)[1][VEC]) const {
-    const uint64_t e = r * cols + c;
-    uint32_t w[4];
-    philox4(M.first() + (e >> 2), M.seed, w);
-    if constexpr (VEC == 4) {  // cols % 4 == 0, so e % 4 == 0
-      const float4 t = ld_stream4(g + e);
-      v[0][0] = M.keep(w[0]) ? t.x * M.factor : 0.0f;
-      v[0][1] = M.keep(w[1]) ? t.y * M.factor : 0.0f;
-      v[0][2] = M.keep(w[2]) ? t.z * M.factor : 0.0f;
-      v[0][3] = M.keep(w[3]) ? t.w * M.factor : 0.0f;
-      if (dx) st_stream4(dx + e, make_float4(v[0][0], v[0][1], v[0][2], v[0][3]));
-    } else {
-      const uint32_t j = (uint32_t)e & 3;
-      const uint32_t word = j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3];
-      v[0][0] = M.keep(word) ? g[e] * M.factor : 0.0f;
-      if (dx) dx[e] = v[0][0];
+// ---- backward with the bias gradient
+// A thread walks down rows with the column sums of one group of four neighbours in registers.  The group
+// is one of the generator's (elements 4 q .. 4 q + 3), so a row costs one generator call and one 16-byte
+// access whatever the width: where cols is no multiple of 4 the groups of row r begin s = r cols mod 4
+// columns to the left of the row's own fours, and a thread takes only rows r + 4 m, for which s, and with
+// it the thread's columns, stay the same.  A warp holds `lx` groups of 32 / lx rows; a CTA `wx` warps side
+// by side (one or two where s is not 0, so that its row step is a multiple of 4) and 8 / wx below each other.
+// A tile of columns is one group narrower than its lanes where s may be 1, 2 or 3.
+//
+// CTAs of a slab of rows write their sums to part[slab]; dropout_bias_kernel adds the slabs up in order.
+constexpr int kDropBwdUnroll = 4;  // rows in flight per thread
+
+struct DropBwdPlan {
+  uint32_t lx, wx;       // lanes per row of a warp; warps side by side
+  uint32_t tile, tiles;  // columns of a CTA; CTAs across
+  uint32_t slabs;
+  uint64_t rows_per_slab;
+};
+
+static DropBwdPlan drop_bwd_plan(uint64_t rows, uint64_t cols) {
+  DropBwdPlan p;
+  const bool even = cols % 4 == 0;
+  const uint64_t groups = even ? cols / 4 : (cols + 2) / 4 + 1;  // of one row, at most
+  p.lx = 1;
+  while (p.lx < 32 && p.lx < groups) p.lx <<= 1;
+  const uint64_t warp_cols = 4ull * (even || groups <= 32 ? p.lx : p.lx - 1);
+  p.wx = 1;
+  while (p.wx < (even ? 8u : 2u) && p.wx * warp_cols < cols) p.wx <<= 1;
+  p.tile = (uint32_t)(p.wx * warp_cols);
+  p.tiles = (uint32_t)((cols + p.tile - 1) / p.tile);
+  const uint64_t step = 8 / p.wx * (32 / p.lx), target = (uint64_t)device_info().sm_count * 6;
+  uint64_t slabs = (target + p.tiles - 1) / p.tiles;
+  const uint64_t most = rows / (step * kDropBwdUnroll) + 1;  // a slab fills a thread's loads once
+  if (slabs > most) slabs = most;
+  p.rows_per_slab = (rows + slabs - 1) / slabs;
+  p.slabs = (uint32_t)((rows + p.rows_per_slab - 1) / p.rows_per_slab);
+  return p;
+}
+
+template <bool VEC, bool DX>
+__global__ void __launch_bounds__(kDropThreads, 4)
+dropout_bwd_kernel(const float* g, uint64_t rows, uint64_t cols, const __grid_constant__ DropBwdPlan P, DropMask M,
+                   float* dx, float* __restrict__ sums) {
+  pdl_trigger();
+  __shared__ float sm[kDropThreads / 32][128 + 4];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t li = lane & (P.lx - 1), sub = lane / P.lx, rpw = 32 / P.lx;
+  const uint32_t wx = warp & (P.wx - 1), wy = warp / P.wx, step = 8 / P.wx * rpw;
+  const uint32_t tile = blockIdx.x % P.tiles, slab = blockIdx.x / P.tiles;
+  const uint32_t warp_cols = P.tile / P.wx;
+  const uint64_t c0 = (uint64_t)tile * P.tile + wx * warp_cols;  // columns [c0, c1) are this warp's
+  const uint64_t c1 = c0 + warp_cols < cols ? c0 + warp_cols : cols;
+  const uint64_t n = rows * cols, first = M.first();
+  const uint64_t r0 = (uint64_t)slab * P.rows_per_slab + wy * rpw + sub;
+  const uint64_t r1 = (uint64_t)(slab + 1) * P.rows_per_slab < rows ? (uint64_t)(slab + 1) * P.rows_per_slab : rows;
+  const uint32_t s = (uint32_t)(r0 * cols) & 3;
+  const int64_t c = (int64_t)(c0 + 4 * li) - s;  // column of the group's first element; c0 is a multiple of 4
+  uint32_t mine = 0;                             // which of the four are this warp's
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j >= (int64_t)c0 && c + j < (int64_t)c1) mine |= 1u << j;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (mine) {
+    // element of the group's first member in row r0; n - 1 is the last there is
+    uint64_t e = r0 * cols + (uint64_t)c;
+    const uint64_t down = (uint64_t)step * cols;
+    for (uint64_t r = r0; r < r1; r += (uint64_t)step * kDropBwdUnroll) {
+      float v[kDropBwdUnroll][4];
+#pragma unroll
+      for (int u = 0; u < kDropBwdUnroll; ++u) {
+        const uint64_t at = e + u * down;
+        if (r + (uint64_t)u * step < r1) {
+          if (VEC && at + 4 <= n) {
+            const float4 t = ld_stream4(g + at);
+            v[u][0] = t.x; v[u][1] = t.y; v[u][2] = t.z; v[u][3] = t.w;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[u][j] = (mine >> j) & 1 ? ld_stream(g + at + j) : 0.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kDropBwdUnroll; ++u) {
+        const uint64_t at = e + u * down;
+        if (r + (uint64_t)u * step < r1) {
+          uint32_t w[4];
+          philox4(first + (at >> 2), M.seed, w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[u][j] = M.keep(w[j]) ? v[u][j] * M.factor : 0.0f;
+            acc[j] += v[u][j];
+          }
+          if (DX) {
+            if (VEC && mine == 15u) {
+              st_stream4(dx + at, make_float4(v[u][0], v[u][1], v[u][2], v[u][3]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if ((mine >> j) & 1) st_stream(dx + at + j, v[u][j]);
+            }
+          }
+        }
+      }
+      e += kDropBwdUnroll * down;
     }
   }
-};
+  // Rows of a warp have columns of their own where s is not 0: sums meet in shared memory by column.
+  // One pass per row of the warp, so that a place has one writer at a time and a fixed order.
+  const uint32_t places = 4 * P.lx;  // at most this many columns
+  for (uint32_t i = lane; i < places; i += 32) sm[warp][i] = 0.0f;
+  for (uint32_t q = 0; q < rpw; ++q) {
+    __syncwarp();
+    if (sub == q) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((mine >> j) & 1) sm[warp][(uint32_t)(c + j - (int64_t)c0)] += acc[j];
+    }
+  }
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < P.tile; i += kDropThreads) {
+    const uint32_t w = i / warp_cols, k = i - w * warp_cols;
+    const uint64_t col = (uint64_t)tile * P.tile + i;
+    if (col < cols) {
+      float t = 0.0f;
+      for (uint32_t y = w; y < 8; y += P.wx) t += sm[y][k];
+      sums[(uint64_t)slab * cols + col] = t;
+    }
+  }
+}
+
+// dbias[c] = sum over slabs of part[slab][c]: eight threads per column take every eighth slab, then a
+// fixed order.
+__global__ void __launch_bounds__(256)
+dropout_bias_kernel(const float* __restrict__ part, uint32_t slabs, uint64_t cols, float* __restrict__ dbias) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float sm[8][32];
+  const uint32_t lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
+  float t = 0.0f;
+  if (c < cols) {
+    uint32_t s = y;
+    for (; s + 24 < slabs; s += 32) {
+      const float a = __ldcg(part + (uint64_t)s * cols + c), b = __ldcg(part + (uint64_t)(s + 8) * cols + c);
+      const float d = __ldcg(part + (uint64_t)(s + 16) * cols + c), f = __ldcg(part + (uint64_t)(s + 24) * cols + c);
+      t = (((t + a) + b) + d) + f;
+    }
+    for (; s < slabs; s += 8) t += __ldcg(part + (uint64_t)s * cols + c);
+  }
+  sm[y][lane] = t;
+  __syncthreads();
+  if (y == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += sm[i][lane];
+    dbias[c] = t;
+  }
+}
 
 __global__ void dropout_advance_kernel(int64_t* counter, uint64_t n) {
   if (threadIdx.x == 0) counter[0] = (int64_t)((uint64_t)counter[0] + n);
@@ -191,10 +321,9 @@ int fb_dropout_fwd(fb_stream_t stream, const float* x, const float* bias, const 
 
 uint64_t fb_dropout_bwd_workspace_bytes(uint64_t rows, uint64_t cols) {
   uint64_t n;
-  if (mul_overflows(rows, cols, &n) || n == 0) return 0;
-  const uint64_t a = col_scratch_bytes(col_plan(1, rows, cols, true), 1, cols, 1);
-  const uint64_t b = col_scratch_bytes(col_plan(1, rows, cols, false), 1, cols, 1);
-  return a > b ? a : b;
+  if (mul_overflows(rows, cols, &n) || n == 0 || cols >= (1ull << 31)) return 0;
+  const DropBwdPlan p = drop_bwd_plan(rows, cols);
+  return p.slabs > 1 ? (uint64_t)p.slabs * cols * sizeof(float) : 0;
 }
 
 int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t cols, float p, uint64_t seed,
@@ -210,9 +339,25 @@ int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t c
   if (!g) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (!dx && !dbias) return FB_OK;
   if (!dbias) return run_dropout(stream, name, g, nullptr, nullptr, n, cols, m, dx);
-  const DropBwdSrc src{g, dx, cols, m};
-  const bool al = aligned16(g) && (!dx || aligned16(dx));
-  return run_col_sum<1>(stream, src, 1, rows, cols, al, dbias, nullptr, 1.0f, workspace, workspace_bytes, name);
+  if (cols >= (1ull << 31)) return fail(FB_ERR_UNSUPPORTED, "%s: a bias of 2^31 or more elements is not supported", name);
+  const DropBwdPlan plan = drop_bwd_plan(rows, cols);
+  const uint64_t need = fb_dropout_bwd_workspace_bytes(rows, cols);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(FB_ERR_WORKSPACE, "%s: needs %llu bytes of scratch", name, (unsigned long long)need);
+  float* sums = plan.slabs > 1 ? static_cast<float*>(workspace) : dbias;
+  const unsigned grid = plan.tiles * plan.slabs;
+  const bool vec = aligned16(g) && (!dx || aligned16(dx));
+  if (vec && dx) dropout_bwd_kernel<true, true><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
+  else if (vec) dropout_bwd_kernel<true, false><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
+  else if (dx) dropout_bwd_kernel<false, true><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
+  else dropout_bwd_kernel<false, false><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
+  FB_LAUNCHED(name);
+  if (plan.slabs > 1) {
+    FB_CUDA(launch_pdl(dropout_bias_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, stream, (const float*)sums,
+                       plan.slabs, cols, dbias));
+    FB_LAUNCHED(name);
+  }
+  return FB_OK;
 }
 
 int fb_dropout_advance(fb_stream_t stream, int64_t* counter, uint64_t n) {

@@ -167,7 +167,8 @@ def test_rope_refusals_of_the_mirror(be):
 
 # ---- dropout ---------------------------------------------------------------------------------------------------------
 
-DROP_SHAPES = [(1, 1), (1, 3), (3, 5), (2, 4), (64, 256), (17, 1001), (5, 4100), (1000, 7), (333, 64), (4099, 33), (1, 100003)]
+DROP_SHAPES = [(1, 1), (1, 3), (3, 5), (2, 4), (64, 256), (17, 1001), (5, 4100), (1000, 7), (333, 64), (4099, 33), (1, 100003), (300, 2050),
+               (9, 121), (9, 122), (9, 123), (9, 124), (9, 126), (40, 127), (50, 249), (50, 497), (700, 6), (20000, 1), (5000, 2), (513, 1030)]
 
 
 @pytest.mark.parametrize("rows,cols", DROP_SHAPES)
