@@ -24,10 +24,9 @@ struct DropMask {
   uint64_t seed, offset;
   const int64_t* counter;
   uint32_t least;  // smallest word that keeps its element
-  int none;        // p == 1: nothing is kept
   float factor;    // 1 / (1 - p)
   __device__ __forceinline__ uint64_t first() const { return offset + (counter ? (uint64_t)__ldg(counter) : 0ull); }
-  __device__ __forceinline__ bool keep(uint32_t word) const { return word >= least && !none; }
+  __device__ __forceinline__ bool keep(uint32_t word) const { return word >= least; }
 };
 
 enum { DROP_NO_BIAS = 0, DROP_BIAS_VEC = 1, DROP_BIAS_SCALAR = 2 };
@@ -99,139 +98,193 @@ dropout_kernel(const float* x, const float* __restrict__ bias, const float* resi
 }
 
 // ---- backward with the bias gradient
-// A thread walks down rows with the column sums of one group of four neighbours in registers.  The group
-// is one of the generator's (elements 4 q .. 4 q + 3), so a row costs one generator call and one 16-byte
-// access whatever the width: where cols is no multiple of 4 the groups of row r begin s = r cols mod 4
-// columns to the left of the row's own fours, and a thread takes only rows r + 4 m, for which s, and with
-// it the thread's columns, stay the same.  A warp holds `lx` groups of 32 / lx rows; a CTA `wx` warps side
-// by side (one or two where s is not 0, so that its row step is a multiple of 4) and 8 / wx below each other.
-// A tile of columns is one group narrower than its lanes where s may be 1, 2 or 3.
+// The tensor is walked flat, in periods of P elements, P a multiple of cols and of 4: a thread that takes
+// the same group of four in every period meets the same columns each time and keeps their sums in
+// registers, whatever the width, with one generator call and one 16-byte access per four elements.  A CTA
+// takes 1024 neighbouring places of the period (a tile) in a slab of periods; P is the multiple of
+// lcm(cols, 4) that fills its last tile best.
 //
-// CTAs of a slab of rows write their sums to part[slab]; dropout_bias_kernel adds the slabs up in order.
-constexpr int kDropBwdUnroll = 4;  // rows in flight per thread
+// What a CTA leaves behind is, for cols >= 1024, its tile of a row of P sums, which is P / cols rows of
+// cols; for fewer columns it first adds up the places of a column and leaves one row.  dropout_bias_kernel
+// adds the rows in order.
+//
+// Bound by HBM as far as a grid of resident CTAs allows that reads and writes in equal measure: 16384 x
+// 4096 in 96 us, 85 % of the copy rate.  Eight groups are in flight per thread while eight go through the
+// generator, on two CTAs per SM; four on three, four or five CTAs took 103 to 125 us, without the early
+// loads 109 us at best, a column sum that draws the mask at each load 107 us.
+constexpr int kDropBwdUnroll = 8;      // groups in flight per thread
+constexpr int kDropBwdPerSm = 2;       // CTAs, by registers
+constexpr uint32_t kDropTile = kDropThreads * 4;
 
 struct DropBwdPlan {
-  uint32_t lx, wx;       // lanes per row of a warp; warps side by side
-  uint32_t tile, tiles;  // columns of a CTA; CTAs across
-  uint32_t slabs;
-  uint64_t rows_per_slab;
+  uint64_t period, periods;   // elements; how many begin in the tensor
+  uint64_t per_slab;          // periods
+  uint32_t tiles, slabs;
+  uint64_t sum_rows;          // rows of cols partial sums
 };
 
 static DropBwdPlan drop_bwd_plan(uint64_t rows, uint64_t cols) {
   DropBwdPlan p;
-  const bool even = cols % 4 == 0;
-  const uint64_t groups = even ? cols / 4 : (cols + 2) / 4 + 1;  // of one row, at most
-  p.lx = 1;
-  while (p.lx < 32 && p.lx < groups) p.lx <<= 1;
-  const uint64_t warp_cols = 4ull * (even || groups <= 32 ? p.lx : p.lx - 1);
-  p.wx = 1;
-  while (p.wx < (even ? 8u : 2u) && p.wx * warp_cols < cols) p.wx <<= 1;
-  p.tile = (uint32_t)(p.wx * warp_cols);
-  p.tiles = (uint32_t)((cols + p.tile - 1) / p.tile);
-  const uint64_t step = 8 / p.wx * (32 / p.lx), target = (uint64_t)device_info().sm_count * 6;
-  uint64_t slabs = (target + p.tiles - 1) / p.tiles;
-  const uint64_t most = rows / (step * kDropBwdUnroll) + 1;  // a slab fills a thread's loads once
+  const uint64_t n = rows * cols, unit = cols % 4 == 0 ? cols : cols % 2 == 0 ? 2 * cols : 4 * cols;
+  const uint64_t target = (uint64_t)device_info().sm_count * kDropBwdPerSm;  // one wave
+  p.period = unit;
+  double best = 0.0;
+  for (uint64_t m = 1; best < 0.95 && (m <= 16 || unit * m <= kDropTile); ++m) {
+    const uint64_t P = unit * m, tiles = (P + kDropTile - 1) / kDropTile;
+    if (m > 1 && (tiles > target || P > n / kDropBwdUnroll)) break;
+    const double full = (double)P / ((double)tiles * kDropTile);
+    if (full > best + 0.05) {
+      best = full;
+      p.period = P;
+    }
+  }
+  p.periods = (n + p.period - 1) / p.period;
+  p.tiles = (uint32_t)((p.period + kDropTile - 1) / kDropTile);
+  uint64_t slabs = target / p.tiles ? target / p.tiles : 1;
+  const uint64_t most = (p.periods + 3) / 4;  // a few groups per thread at least
   if (slabs > most) slabs = most;
-  p.rows_per_slab = (rows + slabs - 1) / slabs;
-  p.slabs = (uint32_t)((rows + p.rows_per_slab - 1) / p.rows_per_slab);
+  p.per_slab = (p.periods + slabs - 1) / slabs;
+  p.slabs = (uint32_t)((p.periods + p.per_slab - 1) / p.per_slab);
+  p.sum_rows = cols < kDropTile ? (uint64_t)p.tiles * p.slabs : p.period / cols * p.slabs;
   return p;
 }
 
+// One group of four: masked, scaled, added to the column sums.
+__device__ __forceinline__ float4 drop_group(const DropMask& M, uint64_t counter, float4 v, float (&acc)[4]) {
+  uint32_t w[4];
+  philox4(counter, M.seed, w);
+  v.x = M.keep(w[0]) ? v.x * M.factor : 0.0f;
+  v.y = M.keep(w[1]) ? v.y * M.factor : 0.0f;
+  v.z = M.keep(w[2]) ? v.z * M.factor : 0.0f;
+  v.w = M.keep(w[3]) ? v.w * M.factor : 0.0f;
+  acc[0] += v.x;
+  acc[1] += v.y;
+  acc[2] += v.z;
+  acc[3] += v.w;
+  return v;
+}
+// Four elements at p, `have` of which exist (4 outside the tensor's last group).
+template <bool VEC>
+__device__ __forceinline__ float4 drop_load(const float* p, uint32_t have = 4) {
+  if (VEC && have == 4) return ld_stream4(p);
+  return make_float4(ld_stream(p), have > 1 ? ld_stream(p + 1) : 0.0f, have > 2 ? ld_stream(p + 2) : 0.0f, have > 3 ? ld_stream(p + 3) : 0.0f);
+}
+template <bool VEC>
+__device__ __forceinline__ void drop_store(float* p, float4 v, uint32_t have = 4) {
+  if (VEC && have == 4) {
+    st_stream4(p, v);
+  } else {
+    st_stream(p, v.x);
+    if (have > 1) st_stream(p + 1, v.y);
+    if (have > 2) st_stream(p + 2, v.z);
+    if (have > 3) st_stream(p + 3, v.w);
+  }
+}
+
 template <bool VEC, bool DX>
-__global__ void __launch_bounds__(kDropThreads, 4)
-dropout_bwd_kernel(const float* g, uint64_t rows, uint64_t cols, const __grid_constant__ DropBwdPlan P, DropMask M,
+__global__ void __launch_bounds__(kDropThreads, kDropBwdPerSm)
+dropout_bwd_kernel(const float* g, uint64_t n, uint32_t cols, const __grid_constant__ DropBwdPlan P, DropMask M,
                    float* dx, float* __restrict__ sums) {
   pdl_trigger();
-  __shared__ float sm[kDropThreads / 32][128 + 4];
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t li = lane & (P.lx - 1), sub = lane / P.lx, rpw = 32 / P.lx;
-  const uint32_t wx = warp & (P.wx - 1), wy = warp / P.wx, step = 8 / P.wx * rpw;
+  __shared__ __align__(16) float sm[kDropTile];
+  __shared__ float part[kDropThreads];
+  constexpr int U = kDropBwdUnroll;
   const uint32_t tile = blockIdx.x % P.tiles, slab = blockIdx.x / P.tiles;
-  const uint32_t warp_cols = P.tile / P.wx;
-  const uint64_t c0 = (uint64_t)tile * P.tile + wx * warp_cols;  // columns [c0, c1) are this warp's
-  const uint64_t c1 = c0 + warp_cols < cols ? c0 + warp_cols : cols;
-  const uint64_t n = rows * cols, first = M.first();
-  const uint64_t r0 = (uint64_t)slab * P.rows_per_slab + wy * rpw + sub;
-  const uint64_t r1 = (uint64_t)(slab + 1) * P.rows_per_slab < rows ? (uint64_t)(slab + 1) * P.rows_per_slab : rows;
-  const uint32_t s = (uint32_t)(r0 * cols) & 3;
-  const int64_t c = (int64_t)(c0 + 4 * li) - s;  // column of the group's first element; c0 is a multiple of 4
-  uint32_t mine = 0;                             // which of the four are this warp's
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (c + j >= (int64_t)c0 && c + j < (int64_t)c1) mine |= 1u << j;
+  const uint64_t place = (uint64_t)tile * kDropTile + 4 * threadIdx.x;  // in the period
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (mine) {
-    // element of the group's first member in row r0; n - 1 is the last there is
-    uint64_t e = r0 * cols + (uint64_t)c;
-    const uint64_t down = (uint64_t)step * cols;
-    for (uint64_t r = r0; r < r1; r += (uint64_t)step * kDropBwdUnroll) {
-      float v[kDropBwdUnroll][4];
-#pragma unroll
-      for (int u = 0; u < kDropBwdUnroll; ++u) {
-        const uint64_t at = e + u * down;
-        if (r + (uint64_t)u * step < r1) {
-          if (VEC && at + 4 <= n) {
-            const float4 t = ld_stream4(g + at);
-            v[u][0] = t.x; v[u][1] = t.y; v[u][2] = t.z; v[u][3] = t.w;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[u][j] = (mine >> j) & 1 ? ld_stream(g + at + j) : 0.0f;
-          }
-        }
+  const uint64_t i0 = (uint64_t)slab * P.per_slab, i1 = i0 + P.per_slab < P.periods ? i0 + P.per_slab : P.periods;
+  const uint64_t at = i0 * P.period + place;
+  if (place < P.period && at < n) {
+    uint64_t left = i1 - i0;  // groups of this thread; in the last period there may be none, or a short one
+    const uint64_t last = at + (left - 1) * P.period;
+    uint32_t have = 0;
+    if (last + 4 > n) {
+      --left;
+      have = last < n ? (uint32_t)(n - last) : 0;
+    }
+    const float* gp = g + at;
+    float* dp = DX ? dx + at : nullptr;
+    uint64_t ctr = M.first() + (at >> 2);
+    const uint64_t down = P.period, ctr_down = P.period >> 2;
+    auto put = [&](float4 v) {
+      v = drop_group(M, ctr, v, acc);
+      ctr += ctr_down;
+      if (DX) {
+        drop_store<VEC>(dp, v);
+        dp += down;
       }
+    };
+    // The next groups' loads are issued before the present ones go through the generator.
+    float4 v[U];
+    if (left >= U) {
 #pragma unroll
-      for (int u = 0; u < kDropBwdUnroll; ++u) {
-        const uint64_t at = e + u * down;
-        if (r + (uint64_t)u * step < r1) {
-          uint32_t w[4];
-          philox4(first + (at >> 2), M.seed, w);
+      for (int u = 0; u < U; ++u, gp += down) v[u] = drop_load<VEC>(gp);
+      for (left -= U; left >= U; left -= U) {
+        float4 next[U];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v[u][j] = M.keep(w[j]) ? v[u][j] * M.factor : 0.0f;
-            acc[j] += v[u][j];
-          }
-          if (DX) {
-            if (VEC && mine == 15u) {
-              st_stream4(dx + at, make_float4(v[u][0], v[u][1], v[u][2], v[u][3]));
-            } else {
+        for (int u = 0; u < U; ++u, gp += down) next[u] = drop_load<VEC>(gp);
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if ((mine >> j) & 1) st_stream(dx + at + j, v[u][j]);
-            }
-          }
-        }
+        for (int u = 0; u < U; ++u) put(v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = next[u];
       }
-      e += kDropBwdUnroll * down;
+      float4 rest[U - 1];
+#pragma unroll
+      for (int u = 0; u < U - 1; ++u)
+        if (u < (int)left) rest[u] = drop_load<VEC>(gp + u * down);
+#pragma unroll
+      for (int u = 0; u < U; ++u) put(v[u]);
+#pragma unroll
+      for (int u = 0; u < U - 1; ++u)
+        if (u < (int)left) put(rest[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U - 1; ++u)
+        if (u < (int)left) v[u] = drop_load<VEC>(gp + u * down);
+#pragma unroll
+      for (int u = 0; u < U - 1; ++u)
+        if (u < (int)left) put(v[u]);
+    }
+    if (have) {  // the tensor's last group, whole or short
+      const float4 w = drop_group(M, M.first() + (last >> 2), drop_load<VEC>(g + last, have), acc);
+      if (DX) drop_store<VEC>(dx + last, w, have);
     }
   }
-  // Rows of a warp have columns of their own where s is not 0: sums meet in shared memory by column.
-  // One pass per row of the warp, so that a place has one writer at a time and a fixed order.
-  const uint32_t places = 4 * P.lx;  // at most this many columns
-  for (uint32_t i = lane; i < places; i += 32) sm[warp][i] = 0.0f;
-  for (uint32_t q = 0; q < rpw; ++q) {
-    __syncwarp();
-    if (sub == q) {
+  if (cols >= kDropTile) {  // places of a tile are different columns
+    if (place < P.period) {
+      float* to = sums + (uint64_t)slab * P.period + place;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if ((mine >> j) & 1) sm[warp][(uint32_t)(c + j - (int64_t)c0)] += acc[j];
+      for (int j = 0; j < 4; ++j) to[j] = acc[j];
     }
+    return;
   }
+  *reinterpret_cast<float4*>(sm + 4 * threadIdx.x) = make_float4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < P.tile; i += kDropThreads) {
-    const uint32_t w = i / warp_cols, k = i - w * warp_cols;
-    const uint64_t col = (uint64_t)tile * P.tile + i;
-    if (col < cols) {
+  // Column c's places in the tile are first, first + cols, ...; `share` threads take them in turn.
+  const uint32_t begin = (uint32_t)(((uint64_t)tile * kDropTile) % cols);
+  const uint32_t share = cols < kDropThreads ? kDropThreads / cols : 1;
+  float* row = sums + (uint64_t)blockIdx.x * cols;
+  for (uint32_t k = threadIdx.x; k < cols * share; k += kDropThreads) {
+    const uint32_t c = k % cols, q = k / cols, first = c >= begin ? c - begin : c + cols - begin;
+    float t = 0.0f;
+    for (uint32_t i = first + q * cols; i < kDropTile; i += share * cols) t += sm[i];  // places behind the period hold 0
+    if (share == 1) row[c] = t;
+    else part[k] = t;
+  }
+  if (share > 1) {
+    __syncthreads();
+    if (threadIdx.x < cols) {
       float t = 0.0f;
-      for (uint32_t y = w; y < 8; y += P.wx) t += sm[y][k];
-      sums[(uint64_t)slab * cols + col] = t;
+      for (uint32_t q = 0; q < share; ++q) t += part[q * cols + threadIdx.x];
+      row[threadIdx.x] = t;
     }
   }
 }
 
-// dbias[c] = sum over slabs of part[slab][c]: eight threads per column take every eighth slab, then a
-// fixed order.
+// dbias[c] = sum over rows of part[row][c]: eight threads per column take every eighth row, then a fixed
+// order.
 __global__ void __launch_bounds__(256)
-dropout_bias_kernel(const float* __restrict__ part, uint32_t slabs, uint64_t cols, float* __restrict__ dbias) {
+dropout_bias_kernel(const float* __restrict__ part, uint32_t rows, uint64_t cols, float* __restrict__ dbias) {
   pdl_wait();
   pdl_trigger();
   __shared__ float sm[8][32];
@@ -240,12 +293,12 @@ dropout_bias_kernel(const float* __restrict__ part, uint32_t slabs, uint64_t col
   float t = 0.0f;
   if (c < cols) {
     uint32_t s = y;
-    for (; s + 24 < slabs; s += 32) {
+    for (; s + 24 < rows; s += 32) {
       const float a = __ldcg(part + (uint64_t)s * cols + c), b = __ldcg(part + (uint64_t)(s + 8) * cols + c);
       const float d = __ldcg(part + (uint64_t)(s + 16) * cols + c), f = __ldcg(part + (uint64_t)(s + 24) * cols + c);
       t = (((t + a) + b) + d) + f;
     }
-    for (; s < slabs; s += 8) t += __ldcg(part + (uint64_t)s * cols + c);
+    for (; s < rows; s += 8) t += __ldcg(part + (uint64_t)s * cols + c);
   }
   sm[y][lane] = t;
   __syncthreads();
@@ -260,12 +313,13 @@ __global__ void dropout_advance_kernel(int64_t* counter, uint64_t n) {
   if (threadIdx.x == 0) counter[0] = (int64_t)((uint64_t)counter[0] + n);
 }
 
-static int make_mask(const char* name, float p, uint64_t seed, uint64_t offset, const int64_t* counter, DropMask* m) {
+// *none: p is 1 (or rounds to it), nothing is kept; no kernel is needed for that.
+static int make_mask(const char* name, float p, uint64_t seed, uint64_t offset, const int64_t* counter, DropMask* m, bool* none) {
   if (!(p >= 0.0f && p <= 1.0f)) return fail(FB_ERR_INVALID_ARG, "%s: p must lie in [0, 1]", name);
   const double t = std::nearbyint((double)p * 4294967296.0);
-  m->none = t >= 4294967296.0;
-  m->least = m->none ? 0xffffffffu : (uint32_t)t;
-  m->factor = m->none ? 0.0f : (float)(1.0 / (1.0 - (double)p));
+  *none = t >= 4294967296.0;
+  m->least = *none ? 0u : (uint32_t)t;
+  m->factor = *none ? 0.0f : (float)(1.0 / (1.0 - (double)p));
   m->seed = seed;
   m->offset = offset;
   m->counter = counter;
@@ -310,12 +364,14 @@ int fb_dropout_fwd(fb_stream_t stream, const float* x, const float* bias, const 
                    uint64_t cols, float p, uint64_t seed, uint64_t offset, const int64_t* counter, float* out) {
   const char* name = "fb_dropout_fwd";
   DropMask m;
-  if (int rc = make_mask(name, p, seed, offset, counter, &m)) return rc;
+  bool none;
+  if (int rc = make_mask(name, p, seed, offset, counter, &m, &none)) return rc;
   uint64_t n;
   if (mul_overflows(rows, cols, &n) || n > (UINT64_MAX >> 3)) return fail(FB_ERR_INVALID_SHAPE, "%s: rows * cols overflows", name);
   if (n == 0) return FB_OK;
   if (!x || !out) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (bias && cols >= (1ull << 31)) return fail(FB_ERR_UNSUPPORTED, "%s: a bias of 2^31 or more elements is not supported", name);
+  if (none) return !residual ? fb_fill(stream, out, 0.0f, n) : out == residual ? FB_OK : fb_copy(stream, out, residual, n);
   return run_dropout(stream, name, x, bias, residual, n, cols, m, out);
 }
 
@@ -323,7 +379,7 @@ uint64_t fb_dropout_bwd_workspace_bytes(uint64_t rows, uint64_t cols) {
   uint64_t n;
   if (mul_overflows(rows, cols, &n) || n == 0 || cols >= (1ull << 31)) return 0;
   const DropBwdPlan p = drop_bwd_plan(rows, cols);
-  return p.slabs > 1 ? (uint64_t)p.slabs * cols * sizeof(float) : 0;
+  return p.sum_rows > 1 ? p.sum_rows * cols * sizeof(float) : 0;
 }
 
 int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t cols, float p, uint64_t seed,
@@ -331,30 +387,36 @@ int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t c
                    uint64_t workspace_bytes) {
   const char* name = "fb_dropout_bwd";
   DropMask m;
-  if (int rc = make_mask(name, p, seed, offset, counter, &m)) return rc;
+  bool none;
+  if (int rc = make_mask(name, p, seed, offset, counter, &m, &none)) return rc;
   uint64_t n;
   if (mul_overflows(rows, cols, &n) || n > (UINT64_MAX >> 3)) return fail(FB_ERR_INVALID_SHAPE, "%s: rows * cols overflows", name);
   if (cols == 0) return FB_OK;
   if (rows == 0) return dbias ? fb_fill(stream, dbias, 0.0f, cols) : FB_OK;
   if (!g) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (!dx && !dbias) return FB_OK;
+  if (none) {
+    if (dx)
+      if (int rc = fb_fill(stream, dx, 0.0f, n)) return rc;
+    return dbias ? fb_fill(stream, dbias, 0.0f, cols) : FB_OK;
+  }
   if (!dbias) return run_dropout(stream, name, g, nullptr, nullptr, n, cols, m, dx);
   if (cols >= (1ull << 31)) return fail(FB_ERR_UNSUPPORTED, "%s: a bias of 2^31 or more elements is not supported", name);
   const DropBwdPlan plan = drop_bwd_plan(rows, cols);
   const uint64_t need = fb_dropout_bwd_workspace_bytes(rows, cols);
   if (need && (!workspace || workspace_bytes < need))
     return fail(FB_ERR_WORKSPACE, "%s: needs %llu bytes of scratch", name, (unsigned long long)need);
-  float* sums = plan.slabs > 1 ? static_cast<float*>(workspace) : dbias;
+  float* sums = need ? static_cast<float*>(workspace) : dbias;
   const unsigned grid = plan.tiles * plan.slabs;
   const bool vec = aligned16(g) && (!dx || aligned16(dx));
-  if (vec && dx) dropout_bwd_kernel<true, true><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
-  else if (vec) dropout_bwd_kernel<true, false><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
-  else if (dx) dropout_bwd_kernel<false, true><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
-  else dropout_bwd_kernel<false, false><<<grid, kDropThreads, 0, stream>>>(g, rows, cols, plan, m, dx, sums);
+  if (vec && dx) dropout_bwd_kernel<true, true><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
+  else if (vec) dropout_bwd_kernel<true, false><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
+  else if (dx) dropout_bwd_kernel<false, true><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
+  else dropout_bwd_kernel<false, false><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
   FB_LAUNCHED(name);
-  if (plan.slabs > 1) {
+  if (need) {
     FB_CUDA(launch_pdl(dropout_bias_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, stream, (const float*)sums,
-                       plan.slabs, cols, dbias));
+                       (uint32_t)plan.sum_rows, cols, dbias));
     FB_LAUNCHED(name);
   }
   return FB_OK;
