@@ -214,6 +214,11 @@ class DeviceBuffer:
         return self.t.dtype == torch.int64
 
 
+_RopeShape = C.c_uint64 * _lib.MAX_RANK
+_RopeStrides = C.c_int64 * _lib.MAX_RANK
+_OutStrides = C.c_int64 * 4
+
+
 def _u64s(vals):
     vals = [int(v) for v in vals]
     return (C.c_uint64 * max(len(vals), 1))(*vals)
@@ -242,13 +247,14 @@ class CudaBackend:
         torch.cuda.set_device(self.device)
         # One non-default stream per backend, like lib.rs:308-312.
         self.stream = torch.cuda.Stream(device=self.device)
+        self._stream_handle = C.c_void_p(self.stream.cuda_stream)
         self._ws = None
         with torch.cuda.stream(self.stream):
             self._bad_expert = torch.zeros(1, dtype=torch.int64, device=self.device)  # see check_experts
 
     # -- plumbing ---------------------------------------------------------------
     def _s(self):
-        return C.c_void_p(self.stream.cuda_stream)
+        return self._stream_handle
 
     def _check(self, rc):
         if rc != 0:
@@ -891,23 +897,28 @@ class CudaBackend:
 
     # -- what a transformer layer runs between its matrix products: shared checks -----------------------
     def _want(self, what, buf, n, i64=False):
-        """`buf` is n elements of f32 (i64) on this device; None passes."""
+        """Address of `buf` after checking that it is n elements of f32 (i64) on this device; None passes."""
         if buf is None:
             return None
-        if buf.device != self.device:
+        t = buf.t
+        if t.get_device() != self.device.index:
             raise Unsupported("buffer belongs to another device")
-        if buf.is_i64 != i64:
+        if t.dtype is not (torch.int64 if i64 else torch.float32):
             raise Unsupported(f"{what} must be an {'i64' if i64 else 'f32'} buffer")
-        if len(buf) != n:
-            raise InvalidShape(f"{what} has {len(buf)} elements, expected {n}")
-        return buf.ptr
+        if t.numel() != n:
+            raise InvalidShape(f"{what} has {t.numel()} elements, expected {n}")
+        return t.data_ptr() if n else None
 
     def _scratch(self, nbytes):
-        """Scratch of one call: stream-ordered, and inside a capture owned by the graph's own pool."""
+        """(address, bytes, owner) of one call's scratch: the backend's own on its stream, but memory of the graph's pool
+        during a capture, so that graphs share none with each other or with eager calls."""
         if not nbytes:
-            return None
-        with torch.cuda.stream(self.stream):
-            return torch.empty(int(nbytes), dtype=torch.uint8, device=self.device)
+            return None, 0, None
+        if torch.cuda.is_current_stream_capturing():
+            with torch.cuda.stream(self.stream):
+                t = torch.empty(int(nbytes), dtype=torch.uint8, device=self.device)
+            return t.data_ptr(), int(nbytes), t
+        return (*self._workspace(nbytes), None)
 
     # -- rotary positions ---------------------------------------------------------------------------------
     ROPE_LAYOUTS = {"interleaved": K.ROPE_INTERLEAVED, "half": K.ROPE_HALF}
@@ -929,35 +940,31 @@ class CudaBackend:
     def _rope(self, x, shape, plan, positions, start, inverse, out):
         if len(shape) != 4:
             raise InvalidShape(f"rope: shape {list(shape)} is not [batch, seq, heads, head_dim]")
-        b, s, h, d = (int(n) for n in shape)
+        b, s, h, d = shape
+        n = b * s * h * d
         row_major = (s * h * d, h * d, d, 1)
         if isinstance(x, DeviceBuffer):
-            if len(x) != b * s * h * d:
-                raise InvalidShape(f"rope: {len(x)} elements for shape {list(shape)}")
+            self._want("rope: x", x, n)
             x = View(x, row_major, 0)
         if out is None:
-            out = self._alloc(b * s * h * d)
+            out = self._alloc(n)
         if isinstance(out, DeviceBuffer):
-            if len(out) != b * s * h * d:
-                raise InvalidShape(f"rope: out has {len(out)} elements for shape {list(shape)}")
+            self._want("rope: out", out, n)
             out = View(out, row_major, 0)
         if len(x.strides) != 4 or len(out.strides) != 4:
             raise InvalidShape("rope: views need four strides")
-        self._own(x.buf, out.buf, plan.turns, positions)
-        if x.buf.is_i64 or out.buf.is_i64:
-            raise Unsupported("rope: x and out must be f32 buffers")
-        rows = 1
+        rows, pp = 1, None
         if positions is not None:
-            if not positions.is_i64:
-                raise Unsupported("rope: positions must be an i64 buffer")
             if len(positions) not in (s, b * s):
                 raise InvalidShape(f"rope: {len(positions)} positions for batch {b} and sequence {s}")
+            pp = self._want("rope: positions", positions, len(positions), i64=True)
             rows = 1 if len(positions) == s else b
-        v = _lib.ViewDesc(x.buf.ptr, len(x.buf), int(x.offset), 4, (C.c_uint64 * _lib.MAX_RANK)(b, s, h, d),
-                          (C.c_int64 * _lib.MAX_RANK)(*x.strides))
-        self._check(self.lib.fb_rope(self._s(), C.byref(v), positions.ptr if positions is not None else None, rows,
-                                     int(start), plan.turns.ptr, plan.rot_dim, plan.layout, plan.scale, inverse,
-                                     out.buf.ptr, len(out.buf), (C.c_int64 * 4)(*out.strides), int(out.offset)))
+        nx, no = len(x.buf), len(out.buf)
+        v = _lib.ViewDesc(self._want("rope: x", x.buf, nx), nx, x.offset, 4, _RopeShape(b, s, h, d), _RopeStrides(*x.strides))
+        self._check(self.lib.fb_rope(self._stream_handle, C.byref(v), pp, rows, start,
+                                     self._want("rope: frequencies", plan.turns, plan.rot_dim // 2, i64=True), plan.rot_dim,
+                                     plan.layout, plan.scale, inverse, self._want("rope: out", out.buf, no), no,
+                                     _OutStrides(*out.strides), out.offset))
         return out.buf
 
     def rope_dev(self, x, shape, plan: RopePlan, positions: Optional[DeviceBuffer] = None, start=0, out=None) -> DeviceBuffer:
@@ -999,11 +1006,10 @@ class CudaBackend:
             dx = self._alloc(n)
         if dbias is None and want_dbias:
             dbias = self._alloc(cols)
-        ws = self._scratch(self.lib.fb_dropout_bwd_workspace_bytes(rows, cols) if dbias is not None else 0)
+        ws, nb, hold = self._scratch(self.lib.fb_dropout_bwd_workspace_bytes(rows, cols) if dbias is not None else 0)
         self._check(self.lib.fb_dropout_bwd(self._s(), pg, rows, cols, p, seed, offset, pc,
                                             self._want("dropout_backward: dx", dx, n),
-                                            self._want("dropout_backward: dbias", dbias, cols),
-                                            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0))
+                                            self._want("dropout_backward: dbias", dbias, cols), ws, nb))
         return dx, dbias
 
     def dropout_advance_dev(self, counter: DeviceBuffer, n):
@@ -1046,11 +1052,11 @@ class CudaBackend:
             order = self._alloc(n, torch.int64)
         if offsets is None:
             offsets = self._alloc(experts + 1, torch.int64)
-        ws = self._scratch(self.lib.fb_moe_sort_workspace_bytes(n, experts))
+        ws, nb, hold = self._scratch(self.lib.fb_moe_sort_workspace_bytes(n, experts))
         self._check(self.lib.fb_moe_sort(self._s(), pi, n, experts, self._want("moe_sort: place", place, n, i64=True),
                                          self._want("moe_sort: order", order, n, i64=True),
-                                         self._want("moe_sort: offsets", offsets, experts + 1, i64=True), self._bad_expert.data_ptr(),
-                                         ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0))
+                                         self._want("moe_sort: offsets", offsets, experts + 1, i64=True),
+                                         self._bad_expert.data_ptr(), ws, nb))
         return MoePlan(place, order, offsets, int(tokens), int(k), int(experts))
 
     def check_experts(self):
