@@ -415,29 +415,41 @@ moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict_
 // warp the rank of an assignment among those of its expert comes from the lanes that hold the same id
 // (match) plus the warp's running count; between warps and chunks counts are summed in order.
 constexpr int kSortThreads = 1024;
-constexpr int kSortRounds = 4;
-constexpr uint32_t kSortChunk = kSortThreads * kSortRounds;
+constexpr int kSortRounds = 4;  // R where one assignment per thread would take too many chunks
 
 __device__ __forceinline__ uint32_t sort_id(int64_t e, uint32_t experts) {
   return e >= 0 && e < (int64_t)experts ? (uint32_t)e : experts;  // `experts`: goes nowhere
 }
 
+// Lanes that hold the same id, by one ballot per bit: 10.3 us for 4096 assignments to 128 experts in one
+// CTA, where the match instruction, which grows with the number of different ids, takes 12.3 us.
+__device__ __forceinline__ uint32_t lanes_alike(uint32_t id, int bits) {
+  uint32_t same = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (id >> b) & 1;
+    const uint32_t v = __ballot_sync(0xffffffffu, set);
+    same &= set ? v : ~v;
+  }
+  return same;
+}
+
 // counts[b][e] = how many assignments of chunk b go to expert e.
+template <int R>
 __global__ void __launch_bounds__(kSortThreads)
 moe_count_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, uint32_t* __restrict__ counts) {
   pdl_trigger();
   extern __shared__ uint32_t hist[];
-  const uint32_t base = blockIdx.x * kSortChunk;
-  uint32_t id[kSortRounds];
+  const uint32_t base = blockIdx.x * (kSortThreads * R);
+  uint32_t id[R];
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r) {
+  for (int r = 0; r < R; ++r) {
     const uint32_t i = base + r * kSortThreads + threadIdx.x;
     id[r] = i < n ? sort_id(__ldg(ids + i), experts) : experts;
   }
   for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) hist[e] = 0;
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kSortRounds; ++r)
+  for (int r = 0; r < R; ++r)
     if (id[r] < experts) atomicAdd(&hist[id[r]], 1u);
   __syncthreads();
   for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) counts[(uint64_t)blockIdx.x * experts + e] = hist[e];
@@ -506,9 +518,10 @@ moe_place_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
   __syncthreads();
   // ranks within the warp
   uint32_t* mine = hist + warp * stride;
+  const int bits = 32 - __clz(experts);  // of the largest id, `experts`
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const uint32_t same = __match_any_sync(0xffffffffu, id[r]);
+    const uint32_t same = lanes_alike(id[r], bits);
     const uint32_t old = id[r] < experts ? mine[id[r]] : 0u;
     rank[r] = old + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
@@ -865,7 +878,22 @@ static int row_vec(uint64_t cols, const void* a, const void* b, const void* c = 
     else { CALL(32); }                             \
   } while (0)
 
-static uint32_t sort_chunks(uint64_t n) { return (uint32_t)((n + kSortChunk - 1) / kSortChunk); }
+// One CTA up to 4096 assignments.  Beyond, chunks of 1024 (a thread each) while their counts can be added up
+// by every CTA, else of 4096: 65536 assignments to 128 experts take 8.3 us in 64 chunks, 15.8 us in 16.
+struct SortPlan {
+  uint32_t rounds, threads, chunks;
+  int mode;
+};
+static SortPlan sort_plan(uint64_t n, uint64_t experts) {
+  SortPlan p;
+  const uint64_t most = n > experts ? n : experts;
+  p.rounds = n <= kSortThreads || (n > kSortThreads * kSortRounds && n <= (uint64_t)kSortThreads * kSortDirect) ? 1 : kSortRounds;
+  p.threads = most < kSortThreads ? (uint32_t)(most + 31) / 32 * 32 : kSortThreads;
+  const uint64_t chunk = (uint64_t)p.threads * p.rounds;
+  p.chunks = n ? (uint32_t)((n + chunk - 1) / chunk) : 1;
+  p.mode = p.chunks == 1 ? SORT_ALONE : p.chunks <= kSortDirect ? SORT_DIRECT : SORT_SCANNED;
+  return p;
+}
 
 }  // namespace fb
 
@@ -918,8 +946,8 @@ int fb_moe_gate_bwd(fb_stream_t stream, const float* dweights, const float* logi
 
 uint64_t fb_moe_sort_workspace_bytes(uint64_t n, uint64_t experts) {
   if (n > 0x7fffffffull || experts == 0 || experts > FB_MOE_MAX_EXPERTS) return 0;
-  const uint64_t chunks = sort_chunks(n);
-  return chunks > 1 ? (chunks + 1) * experts * sizeof(uint32_t) : 0;
+  const SortPlan p = sort_plan(n, experts);
+  return p.chunks > 1 ? ((uint64_t)p.chunks + 1) * experts * sizeof(uint32_t) : 0;
 }
 
 int fb_moe_sort(fb_stream_t stream, const int64_t* ids, uint64_t n, uint64_t experts, int64_t* place, int64_t* order,
@@ -932,30 +960,28 @@ int fb_moe_sort(fb_stream_t stream, const int64_t* ids, uint64_t n, uint64_t exp
   const uint64_t need = fb_moe_sort_workspace_bytes(n, experts);
   if (need && (!workspace || workspace_bytes < need))
     return fail(FB_ERR_WORKSPACE, "%s: needs %llu bytes of scratch", name, (unsigned long long)need);
-  const uint32_t chunks = n ? sort_chunks(n) : 1, E = (uint32_t)experts, n32 = (uint32_t)n;
-  // One CTA with a thread per assignment where that suffices, else kSortRounds per thread.
-  const bool small = n <= kSortThreads;
-  const uint32_t most = n32 > E ? n32 : E, threads = small ? (most + 31) / 32 * 32 : kSortThreads;
-  const size_t smem = (2 * (size_t)E + (size_t)(threads / 32) * (E | 1)) * sizeof(uint32_t);
-  const void* kernel = small ? (const void*)moe_place_kernel<1> : (const void*)moe_place_kernel<kSortRounds>;
-  if (smem > 48 * 1024) FB_CUDA(allow_dyn_smem(kernel, smem));
+  const uint32_t E = (uint32_t)experts, n32 = (uint32_t)n;
+  const SortPlan p = sort_plan(n, experts);
+  const size_t smem = (2 * (size_t)E + (size_t)(p.threads / 32) * (E | 1)) * sizeof(uint32_t);
+  const bool one = p.rounds == 1;
+  if (smem > 48 * 1024) FB_CUDA(allow_dyn_smem(one ? (const void*)moe_place_kernel<1> : (const void*)moe_place_kernel<kSortRounds>, smem));
   uint32_t* counts = static_cast<uint32_t*>(workspace);
-  uint32_t* totals = counts + (uint64_t)chunks * E;
-  const int mode = chunks == 1 ? SORT_ALONE : chunks <= kSortDirect ? SORT_DIRECT : SORT_SCANNED;
-  if (mode == SORT_ALONE) {
-    if (small) moe_place_kernel<1><<<1, threads, smem, stream>>>(ids, n32, E, 1, mode, nullptr, nullptr, place, order, offsets, bad_index);
-    else moe_place_kernel<kSortRounds><<<1, threads, smem, stream>>>(ids, n32, E, 1, mode, nullptr, nullptr, place, order, offsets, bad_index);
+  uint32_t* totals = counts + (uint64_t)p.chunks * E;
+  if (p.mode == SORT_ALONE) {
+    if (one) moe_place_kernel<1><<<1, p.threads, smem, stream>>>(ids, n32, E, 1, p.mode, nullptr, nullptr, place, order, offsets, bad_index);
+    else moe_place_kernel<kSortRounds><<<1, p.threads, smem, stream>>>(ids, n32, E, 1, p.mode, nullptr, nullptr, place, order, offsets, bad_index);
     FB_LAUNCHED(name);
     return FB_OK;
   }
-  moe_count_kernel<<<chunks, kSortThreads, E * sizeof(uint32_t), stream>>>(ids, n32, E, counts);
+  if (one) moe_count_kernel<1><<<p.chunks, kSortThreads, E * sizeof(uint32_t), stream>>>(ids, n32, E, counts);
+  else moe_count_kernel<kSortRounds><<<p.chunks, kSortThreads, E * sizeof(uint32_t), stream>>>(ids, n32, E, counts);
   FB_LAUNCHED(name);
-  if (mode == SORT_SCANNED) {
-    FB_CUDA(launch_pdl(moe_scan_kernel, dim3((E + 31) / 32), dim3(1024), 0, stream, counts, chunks, E, totals));
+  if (p.mode == SORT_SCANNED) {
+    FB_CUDA(launch_pdl(moe_scan_kernel, dim3((E + 31) / 32), dim3(1024), 0, stream, counts, p.chunks, E, totals));
     FB_LAUNCHED(name);
   }
-  FB_CUDA(launch_pdl(moe_place_kernel<kSortRounds>, dim3(chunks), dim3(threads), smem, stream, ids, n32, E, chunks, mode,
-                     (const uint32_t*)counts, (const uint32_t*)totals, place, order, offsets, bad_index));
+  FB_CUDA(launch_pdl(one ? moe_place_kernel<1> : moe_place_kernel<kSortRounds>, dim3(p.chunks), dim3(p.threads), smem, stream, ids,
+                     n32, E, p.chunks, p.mode, (const uint32_t*)counts, (const uint32_t*)totals, place, order, offsets, bad_index));
   FB_LAUNCHED(name);
   return FB_OK;
 }
