@@ -323,12 +323,12 @@ moe_gate_fwd_many_kernel(const float* __restrict__ logits, uint64_t tokens, uint
 // L lanes per token; lane l takes choices l, l + L, ...  The row is laid out in shared memory and the
 // chosen entries written over it.  A chosen entry is w_j (dw_j - sum w dw) in both forms: the saved
 // weight is its probability.
-template <int L, int V>
+template <int L, int V, int MINE>
 __global__ void __launch_bounds__(kGateThreads)
 moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict__ logits, const float* __restrict__ weights,
                     const int64_t* __restrict__ ids, uint64_t tokens, uint32_t experts, uint32_t k, bool renorm, bool vec,
                     float* __restrict__ dlogits) {
-  constexpr int kTokens = 32 / L, kMine = FB_MOE_MAX_K / L;
+  constexpr int kTokens = 32 / L;  // MINE choices a lane
   __shared__ __align__(16) float rows[kGateThreads / L][L * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, g = lane / L;
   float* out = rows[warp * kTokens + g];
@@ -338,10 +338,10 @@ moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict_
     const bool live = t < tokens;
     float v[V];
     if (!renorm) gate_load<L, V>(logits + t * experts, experts, l, vec, live, v);
-    float w[kMine], dw[kMine], dot = 0.0f;
-    int32_t id[kMine];
+    float w[MINE], dw[MINE], dot = 0.0f;
+    int32_t id[MINE];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
+    for (int i = 0; i < MINE; ++i) {
       const uint32_t j = i * L + l;
       id[i] = -1;
       w[i] = dw[i] = 0.0f;
@@ -389,7 +389,7 @@ moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict_
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < kMine; ++i)
+    for (int i = 0; i < MINE; ++i)
       if (id[i] >= 0) out[id[i]] = w[i] * (dw[i] - dot);
     __syncwarp();
     if (live) {
@@ -935,11 +935,16 @@ int fb_moe_gate_bwd(fb_stream_t stream, const float* dweights, const float* logi
   if (tokens == 0) return FB_OK;
   if (!dweights || !weights || !ids || !dlogits || (!renorm && !logits)) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   const bool vec = experts % 4 == 0 && aligned16(dlogits) && (renorm || aligned16(logits));
-#define FB_CALL(L, V)                                                                                            \
-  moe_gate_bwd_kernel<L, V><<<grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L)), kGateThreads, 0, stream>>>( \
+#define FB_CALL(L, V, MINE)                                                                                      \
+  moe_gate_bwd_kernel<L, V, MINE><<<grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L)), kGateThreads, 0, stream>>>( \
       dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, renorm != 0, vec, dlogits)
-  FB_GATE_ROWS(experts, FB_CALL);
+#define FB_CALL1(L, V) FB_CALL(L, V, 1)
+#define FB_CALL_ALL(L, V) FB_CALL(L, V, (FB_MOE_MAX_K / L))
+  if (k <= 8) FB_GATE_ROWS(experts, FB_CALL1);
+  else FB_GATE_ROWS(experts, FB_CALL_ALL);
 #undef FB_CALL
+#undef FB_CALL1
+#undef FB_CALL_ALL
   FB_LAUNCHED(name);
   return FB_OK;
 }

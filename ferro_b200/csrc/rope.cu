@@ -4,12 +4,15 @@
 // Angle.  theta_i is given in turns as a 64-bit fixed-point fraction, so the
 // fraction of a turn at position p is the low 64 bits of p * turns_i: exact
 // integer arithmetic, no range reduction, the same error (|p| * 2^-65 turns) for
-// the first position and the millionth.  Its top 32 bits become a float in
-// [-1, 1) half turns, off by at most 2^-25, which is what sincospif takes.
+// the first position and the millionth.
 //
 // Roofline: HBM, 8 bytes per element.  A thread owns one group of pairs of one
 // token and walks HPT heads with it, so cosine and sine are paid once per HPT
-// heads; all of a thread's loads are issued before the first product.
+// heads; all of a thread's loads are issued before the first product.  Measured
+// against the copy rate: 4 x 4096 tokens of 32 heads of 128 100 % in both layouts
+// (82 us), 64 of 256 channels turned 104 %, 40 of 80 89 to 95 %, 126 channels (no
+// 16-byte access fits) 88 to 96 %, one head 62 to 82 %: bound by the instructions
+// of the angles there.
 #include <cmath>
 
 #include "common.cuh"
@@ -17,7 +20,7 @@
 
 namespace fb {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;  // 256: 2 to 20 % slower throughout
 
 struct RopeArgs {
   const float* x;
@@ -31,10 +34,11 @@ struct RopeArgs {
   uint32_t upt;                // threads per token: head chunks * units
   uint32_t tpb, bpt;           // tokens per CTA; CTAs per token
   uint32_t pos_batch;          // 1: positions have a row per batch entry
-  uint32_t rot;
+  uint32_t rot, dim;
   FastDiv d_upt, d_units, d_seq, d_bpt;
   uint64_t blocks;
-  float scale, sign;
+  float scale;
+  uint32_t flip;               // sign bit where the angle is negated
 };
 
 template <int V>
@@ -55,11 +59,31 @@ __device__ __forceinline__ void rope_store(float* p, const float (&v)[VEC]) {
   __stcs(reinterpret_cast<T*>(p), *reinterpret_cast<const T*>(v));
 }
 
-__device__ __forceinline__ void turn_sincos(uint64_t turns, float scale, float sign, float& s, float& c) {
-  const float h = (float)(int32_t)(turns >> 32) * 4.656612873077393e-10f;  // 2^-31: half turns in [-1, 1]
-  sincospif(h, &s, &c);
-  s *= scale * sign;
-  c *= scale;
+// Cosine and sine of a fraction of a turn (top 32 bits of the fixed-point word), from their Taylor series
+// after the nearest quarter turn is taken off exactly: x, half turns in [-1/4, 1/4], is the integer
+// remainder times a power of two.  The terms left out are below 2e-9 (sine, from x^11) and 2e-10 (cosine,
+// from x^12); pi is kept in two floats, so that what counts is the rounding of x and of the result.
+// About 25 instructions.  Where one head has to pay for them alone (8 x 8192 tokens of 128 channels, half
+// layout) the kernel takes 16.5 us, with sincospif, which reduces a float argument first, 18.6.
+__device__ __forceinline__ void turn_sincos(uint64_t turns, float scale, uint32_t flip, float& s, float& c) {
+  const uint32_t t = (uint32_t)(turns >> 32), q = (t + 0x20000000u) >> 30;
+  const float x = (float)(int32_t)(t - (q << 30)) * 4.656612873077393e-10f;  // 2^-31
+  const float y = x * x;
+  float a = 0.08214588661112822f;  // pi^9 / 9!
+  a = fmaf(a, y, -0.5992645293207921f);
+  a = fmaf(a, y, 2.550164039877345f);
+  a = fmaf(a, y, -5.16771278004997f);
+  a = fmaf(x, 3.1415927410125732f, x * fmaf(a, y, -8.742278e-8f));
+  float b = -0.02580689139001406f;  // -pi^10 / 10!
+  b = fmaf(b, y, 0.23533063035889312f);
+  b = fmaf(b, y, -1.3352627688545893f);
+  b = fmaf(b, y, 4.058712126416768f);
+  b = fmaf(b, y, -4.934802200544679f);
+  b = fmaf(b, y, 1.0f);
+  const bool odd = q & 1;
+  // quarter turns: (c, s) -> (-s, c) each
+  s = (odd ? b : a) * __uint_as_float(__float_as_uint(scale) ^ ((q & 2) << 30) ^ flip);
+  c = (odd ? a : b) * __uint_as_float(__float_as_uint(scale) ^ (((q + 1) & 2) << 30));
 }
 
 // A group of pairs is, in the half layout, VEC neighbours of the first half and the VEC across from
@@ -87,63 +111,71 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
     const uint32_t h0 = chunk * HPT, hn = min((uint32_t)HPT, A.heads - h0);
     const float* xp = A.x + (int64_t)b * A.xs[0] + (int64_t)s * A.xs[1] + (int64_t)h0 * A.xs[2];
     float* op = A.out + (int64_t)b * A.os[0] + (int64_t)s * A.os[1] + (int64_t)h0 * A.os[2];
-    if (u < A.pair_units) {
-      const uint32_t pair = u * kPairs;
-      const uint32_t ca = LAYOUT == FB_ROPE_HALF ? pair : 2 * pair;             // channel of the first vector
-      const uint32_t cb = LAYOUT == FB_ROPE_HALF ? pair + A.half : 2 * pair + 1;  // and of the second
-      float va[HPT][VEC], vb[HPT][VEC];
+    // Groups of copied channels go through the same loads and stores, so that a warp that holds both
+    // kinds waits for memory once.
+    const bool turn = u < A.pair_units;
+    const uint32_t pair = u * kPairs;
+    uint32_t ca, cb;  // channels of the first and, where there is one, the second vector
+    bool second = kTwo;
+    if (turn) {
+      ca = LAYOUT == FB_ROPE_HALF ? pair : 2 * pair;
+      cb = LAYOUT == FB_ROPE_HALF ? pair + A.half : 2 * pair + 1;
+    } else {
+      ca = A.rot + (u - A.pair_units) * (kTwo ? 2 * VEC : VEC);
+      cb = ca + VEC;
+      second = kTwo && cb < A.dim;
+    }
+    const float* xa = xp + (int64_t)ca * A.xs[3];
+    const float* xb = xp + (int64_t)cb * A.xs[3];
+    float va[HPT][VEC], vb[HPT][VEC];
 #pragma unroll
-      for (int h = 0; h < HPT; ++h)
-        if (h < (int)hn) {
-          rope_load<VEC>(xp + (int64_t)h * A.xs[2] + (int64_t)ca * A.xs[3], va[h]);
-          if constexpr (kTwo) rope_load<VEC>(xp + (int64_t)h * A.xs[2] + (int64_t)cb * A.xs[3], vb[h]);
-        }
+    for (int h = 0; h < HPT; ++h)
+      if (h < (int)hn) {
+        rope_load<VEC>(xa + (int64_t)h * A.xs[2], va[h]);
+        if (kTwo && second) rope_load<VEC>(xb + (int64_t)h * A.xs[2], vb[h]);
+      }
+    if (turn) {
       const uint64_t p = A.pos ? (uint64_t)__ldg(A.pos + (A.pos_batch ? token : s)) : (uint64_t)A.start + s;
       float sn[kPairs], cs[kPairs];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) turn_sincos(p * (uint64_t)__ldg(A.turns + pair + i), A.scale, A.sign, sn[i], cs[i]);
+      for (int i = 0; i < kPairs; ++i) turn_sincos(p * (uint64_t)__ldg(A.turns + pair + i), A.scale, A.flip, sn[i], cs[i]);
 #pragma unroll
       for (int h = 0; h < HPT; ++h)
         if (h < (int)hn) {
-          if constexpr (kTwo) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              const float a = va[h][i], c = vb[h][i];
-              va[h][i] = a * cs[i] - c * sn[i];
-              vb[h][i] = c * cs[i] + a * sn[i];
-            }
-            rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)ca * A.os[3], va[h]);
-            rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)cb * A.os[3], vb[h]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i) {
-              const float a = va[h][2 * i], c = va[h][2 * i + 1];
-              va[h][2 * i] = a * cs[i] - c * sn[i];
-              va[h][2 * i + 1] = c * cs[i] + a * sn[i];
-            }
-            rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)ca * A.os[3], va[h]);
+          for (int i = 0; i < kPairs; ++i) {
+            float& a = kTwo ? va[h][i] : va[h][2 * i];
+            float& c = kTwo ? vb[h][i] : va[h][2 * i + 1];
+            const float t = a * cs[i] - c * sn[i];
+            c = c * cs[i] + a * sn[i];
+            a = t;
           }
         }
-    } else {
-      const uint32_t c = A.rot + (u - A.pair_units) * VEC;
-      float v[HPT][VEC];
-#pragma unroll
-      for (int h = 0; h < HPT; ++h)
-        if (h < (int)hn) rope_load<VEC>(xp + (int64_t)h * A.xs[2] + (int64_t)c * A.xs[3], v[h]);
-#pragma unroll
-      for (int h = 0; h < HPT; ++h)
-        if (h < (int)hn) rope_store<VEC>(op + (int64_t)h * A.os[2] + (int64_t)c * A.os[3], v[h]);
     }
+    float* oa = op + (int64_t)ca * A.os[3];
+    float* ob = op + (int64_t)cb * A.os[3];
+#pragma unroll
+    for (int h = 0; h < HPT; ++h)
+      if (h < (int)hn) {
+        rope_store<VEC>(oa + (int64_t)h * A.os[2], va[h]);
+        if (kTwo && second) rope_store<VEC>(ob + (int64_t)h * A.os[2], vb[h]);
+      }
   }
 }
 
 template <int VEC, int LAYOUT>
 static int rope_launch(cudaStream_t stream, RopeArgs& A, bool in_place, uint32_t head_dim) {
   A.pair_units = LAYOUT == FB_ROPE_HALF ? A.half / VEC : (VEC == 1 ? A.half : A.half / (VEC / 2));
-  A.units = A.pair_units + (in_place ? 0 : (head_dim - A.rot) / VEC);
+  constexpr uint32_t kUnit = LAYOUT == FB_ROPE_HALF || VEC == 1 ? 2 * VEC : VEC;  // channels of a group
+  A.units = A.pair_units + (in_place ? 0 : (head_dim - A.rot + kUnit - 1) / kUnit);
+  A.dim = head_dim;
   const uint64_t work = (uint64_t)A.tokens * A.units;
+  // Heads per thread: four share the cost of cosine and sine and keep their loads in flight, as far as
+  // there are heads, and threads enough to fill the SMs.
   const bool few = work * ((A.heads + 3) / 4) < (uint64_t)device_info().sm_count * 2048;
-  const uint32_t hpt = few ? 1 : 4;
+  const uint32_t most = VEC == 4 ? 4 : 8;  // eight where an access is narrower
+  uint32_t hpt = 1;
+  while (!few && hpt < most && hpt < A.heads) hpt <<= 1;
   A.upt = (A.heads + hpt - 1) / hpt * A.units;
   A.tpb = A.upt < kRopeThreads ? kRopeThreads / A.upt : 1;
   A.bpt = A.upt < kRopeThreads ? 1 : (A.upt + kRopeThreads - 1) / kRopeThreads;
@@ -152,8 +184,10 @@ static int rope_launch(cudaStream_t stream, RopeArgs& A, bool in_place, uint32_t
   A.d_seq = make_fastdiv(A.seq);
   A.blocks = (uint64_t)((A.tokens + A.tpb - 1) / A.tpb) * A.bpt;
   const unsigned grid = grid_full(A.blocks);
-  if (few) rope_kernel<VEC, LAYOUT, 1><<<grid, kRopeThreads, 0, stream>>>(A);
-  else rope_kernel<VEC, LAYOUT, 4><<<grid, kRopeThreads, 0, stream>>>(A);
+  if (hpt == 1) rope_kernel<VEC, LAYOUT, 1><<<grid, kRopeThreads, 0, stream>>>(A);
+  else if (hpt == 2) rope_kernel<VEC, LAYOUT, 2><<<grid, kRopeThreads, 0, stream>>>(A);
+  else if (hpt == 4) rope_kernel<VEC, LAYOUT, 4><<<grid, kRopeThreads, 0, stream>>>(A);
+  else if constexpr (VEC < 4) rope_kernel<VEC, LAYOUT, 8><<<grid, kRopeThreads, 0, stream>>>(A);
   FB_LAUNCHED("fb_rope");
   return FB_OK;
 }
@@ -302,7 +336,7 @@ int fb_rope(fb_stream_t stream, const fb_view* x, const int64_t* positions, uint
   A.half = (uint32_t)(rot_dim / 2);
   A.rot = (uint32_t)rot_dim;
   A.scale = scale;
-  A.sign = inverse ? -1.0f : 1.0f;
+  A.flip = inverse ? 0x80000000u : 0u;
   return layout == FB_ROPE_HALF ? rope_vec<FB_ROPE_HALF>(stream, A, in_place, (uint32_t)D, vec)
                                 : rope_vec<FB_ROPE_INTERLEAVED>(stream, A, in_place, (uint32_t)D, vec);
 }

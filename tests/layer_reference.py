@@ -46,11 +46,12 @@ def rope(x, angles, layout, scale=1.0, inverse=False):
 
 
 def rope_bound(x, rot, layout, scale=1.0):
-    """How far one f32 result may be off.  The angle: the fraction of a turn becomes a float of half turns in [-1, 1], off
-    by 2^-25 of a half turn, and 2^-31 of one was cut off before: pi (2^-25 + 2^-31).  sincospif: 2 ulp, 2^-23.  Times
-    scale, each product and the final sum: three roundings of 2^-24.  All of it relative to (|a| + |b|) * scale."""
+    """How far one f32 result may be off.  The angle: its remainder of a quarter turn, at most 1/4 of a half turn, becomes a
+    float, off by 2^-27 of a half turn, after 2^-31 of one was cut off: pi (2^-27 + 2^-31).  Cosine and sine from their
+    series: 2^-23, two units in the last place.  Times scale, each product and the final sum: three roundings of 2^-24.
+    All of it relative to (|a| + |b|) * scale."""
     x = np.abs(np.asarray(x, np.float64))
-    per = math.pi * (2.0 ** -25 + 2.0 ** -31) + 2.0 ** -23 + 3 * EPS
+    per = math.pi * (2.0 ** -27 + 2.0 ** -31) + 2.0 ** -23 + 3 * EPS
     bound = np.zeros_like(x)
     a, b = (slice(0, rot // 2), slice(rot // 2, rot)) if layout == "half" else (slice(0, rot, 2), slice(1, rot, 2))
     bound[..., a] = bound[..., b] = (x[..., a] + x[..., b]) * scale * per
