@@ -909,6 +909,16 @@ class CudaBackend:
             raise InvalidShape(f"{what} has {t.numel()} elements, expected {n}")
         return t.data_ptr() if n else None
 
+    def _call(self, fn, *args):
+        """One library call on this backend's stream, with its device current (another backend's may be)."""
+        if torch.cuda.current_device() == self.device.index:
+            rc = fn(self._stream_handle, *args)
+        else:
+            with torch.cuda.device(self.device):
+                rc = fn(self._stream_handle, *args)
+        if rc != 0:
+            self._check(rc)
+
     def _scratch(self, nbytes):
         """(address, bytes, owner) of one call's scratch: the backend's own on its stream, but memory of the graph's pool
         during a capture, so that graphs share none with each other or with eager calls."""
@@ -961,10 +971,10 @@ class CudaBackend:
             rows = 1 if len(positions) == s else b
         nx, no = len(x.buf), len(out.buf)
         v = _lib.ViewDesc(self._want("rope: x", x.buf, nx), nx, x.offset, 4, _RopeShape(b, s, h, d), _RopeStrides(*x.strides))
-        self._check(self.lib.fb_rope(self._stream_handle, C.byref(v), pp, rows, start,
+        self._call(self.lib.fb_rope, C.byref(v), pp, rows, start,
                                      self._want("rope: frequencies", plan.turns, plan.rot_dim // 2, i64=True), plan.rot_dim,
                                      plan.layout, plan.scale, inverse, self._want("rope: out", out.buf, no), no,
-                                     _OutStrides(*out.strides), out.offset))
+                                     _OutStrides(*out.strides), out.offset)
         return out.buf
 
     def rope_dev(self, x, shape, plan: RopePlan, positions: Optional[DeviceBuffer] = None, start=0, out=None) -> DeviceBuffer:
@@ -993,8 +1003,8 @@ class CudaBackend:
         pc = self._want("dropout: counter", counter, 1, i64=True)
         if out is None:
             out = self._alloc(n)
-        self._check(self.lib.fb_dropout_fwd(self._s(), px, pb, pr, rows, cols, p, seed, offset, pc,
-                                            self._want("dropout: out", out, n)))
+        self._call(self.lib.fb_dropout_fwd, px, pb, pr, rows, cols, p, seed, offset, pc,
+                                            self._want("dropout: out", out, n))
         return out
 
     def dropout_backward_dev(self, g, p, seed, offset, rows, cols, counter: Optional[DeviceBuffer] = None, want_dx=True,
@@ -1007,14 +1017,14 @@ class CudaBackend:
         if dbias is None and want_dbias:
             dbias = self._alloc(cols)
         ws, nb, hold = self._scratch(self.lib.fb_dropout_bwd_workspace_bytes(rows, cols) if dbias is not None else 0)
-        self._check(self.lib.fb_dropout_bwd(self._s(), pg, rows, cols, p, seed, offset, pc,
+        self._call(self.lib.fb_dropout_bwd, pg, rows, cols, p, seed, offset, pc,
                                             self._want("dropout_backward: dx", dx, n),
-                                            self._want("dropout_backward: dbias", dbias, cols), ws, nb))
+                                            self._want("dropout_backward: dbias", dbias, cols), ws, nb)
         return dx, dbias
 
     def dropout_advance_dev(self, counter: DeviceBuffer, n):
         """counter[0] += n on the device: a captured step draws new masks at every replay."""
-        self._check(self.lib.fb_dropout_advance(self._s(), self._want("dropout_advance: counter", counter, 1, i64=True), n))
+        self._call(self.lib.fb_dropout_advance, self._want("dropout_advance: counter", counter, 1, i64=True), n)
 
     # -- routed experts ---------------------------------------------------------------------------------------
     def moe_gate_dev(self, logits, tokens, experts, k, renorm=True, weights=None, ids=None):
@@ -1025,9 +1035,9 @@ class CudaBackend:
             weights = self._alloc(tokens * k)
         if ids is None:
             ids = self._alloc(tokens * k, torch.int64)
-        self._check(self.lib.fb_moe_gate_fwd(self._s(), pl, tokens, experts, k, 1 if renorm else 0,
+        self._call(self.lib.fb_moe_gate_fwd, pl, tokens, experts, k, 1 if renorm else 0,
                                              self._want("moe_gate: weights", weights, tokens * k),
-                                             self._want("moe_gate: ids", ids, tokens * k, i64=True)))
+                                             self._want("moe_gate: ids", ids, tokens * k, i64=True))
         return weights, ids
 
     def moe_gate_backward_dev(self, dweights, logits, weights, ids, tokens, experts, k, renorm=True, dlogits=None) -> DeviceBuffer:
@@ -1037,8 +1047,8 @@ class CudaBackend:
         pi = self._want("moe_gate_backward: ids", ids, tokens * k, i64=True)
         if dlogits is None:
             dlogits = self._alloc(tokens * experts)
-        self._check(self.lib.fb_moe_gate_bwd(self._s(), pd, pl, pw, pi, tokens, experts, k, 1 if renorm else 0,
-                                             self._want("moe_gate_backward: dlogits", dlogits, tokens * experts)))
+        self._call(self.lib.fb_moe_gate_bwd, pd, pl, pw, pi, tokens, experts, k, 1 if renorm else 0,
+                                             self._want("moe_gate_backward: dlogits", dlogits, tokens * experts))
         return dlogits
 
     def moe_sort_dev(self, ids, tokens, k, experts, place=None, order=None, offsets=None) -> MoePlan:
@@ -1053,10 +1063,10 @@ class CudaBackend:
         if offsets is None:
             offsets = self._alloc(experts + 1, torch.int64)
         ws, nb, hold = self._scratch(self.lib.fb_moe_sort_workspace_bytes(n, experts))
-        self._check(self.lib.fb_moe_sort(self._s(), pi, n, experts, self._want("moe_sort: place", place, n, i64=True),
+        self._call(self.lib.fb_moe_sort, pi, n, experts, self._want("moe_sort: place", place, n, i64=True),
                                          self._want("moe_sort: order", order, n, i64=True),
                                          self._want("moe_sort: offsets", offsets, experts + 1, i64=True),
-                                         self._bad_expert.data_ptr(), ws, nb))
+                                         self._bad_expert.data_ptr(), ws, nb)
         return MoePlan(place, order, offsets, int(tokens), int(k), int(experts))
 
     def check_experts(self):
@@ -1082,8 +1092,8 @@ class CudaBackend:
         if out is None:
             out = self._alloc(plan.tokens * plan.k * cols)
         rows = self._moe_rows("moe_dispatch", out, cols)
-        self._check(self.lib.fb_moe_dispatch_fwd(self._s(), px, plan.place.ptr, plan.tokens, plan.k, cols,
-                                                 self._want("moe_dispatch: out", out, rows * cols), rows))
+        self._call(self.lib.fb_moe_dispatch_fwd, px, plan.place.ptr, plan.tokens, plan.k, cols,
+                                                 self._want("moe_dispatch: out", out, rows * cols), rows)
         return out
 
     def moe_dispatch_backward_dev(self, g, plan: MoePlan, cols, out=None) -> DeviceBuffer:
@@ -1092,8 +1102,8 @@ class CudaBackend:
         pg = self._want("moe_dispatch_backward: g", g, rows * cols)
         if out is None:
             out = self._alloc(plan.tokens * cols)
-        self._check(self.lib.fb_moe_dispatch_bwd(self._s(), pg, plan.place.ptr, plan.tokens, plan.k, cols, rows,
-                                                 self._want("moe_dispatch_backward: out", out, plan.tokens * cols)))
+        self._call(self.lib.fb_moe_dispatch_bwd, pg, plan.place.ptr, plan.tokens, plan.k, cols, rows,
+                                                 self._want("moe_dispatch_backward: out", out, plan.tokens * cols))
         return out
 
     def moe_combine_dev(self, ys, weights, plan: MoePlan, cols, out=None) -> DeviceBuffer:
@@ -1102,8 +1112,8 @@ class CudaBackend:
         py, pw = self._want("moe_combine: ys", ys, rows * cols), self._want("moe_combine: weights", weights, plan.tokens * plan.k)
         if out is None:
             out = self._alloc(plan.tokens * cols)
-        self._check(self.lib.fb_moe_combine_fwd(self._s(), py, pw, plan.place.ptr, plan.tokens, plan.k, cols, rows,
-                                                self._want("moe_combine: out", out, plan.tokens * cols)))
+        self._call(self.lib.fb_moe_combine_fwd, py, pw, plan.place.ptr, plan.tokens, plan.k, cols, rows,
+                                                self._want("moe_combine: out", out, plan.tokens * cols))
         return out
 
     def moe_combine_backward_dev(self, g, ys, weights, plan: MoePlan, cols, want_dys=True, want_dweights=True, dys=None,
@@ -1115,8 +1125,8 @@ class CudaBackend:
             dys = self._alloc(rows * cols)
         if dweights is None and want_dweights:
             dweights = self._alloc(plan.tokens * plan.k)
-        self._check(self.lib.fb_moe_combine_bwd(self._s(), pg, self._want("moe_combine_backward: ys", ys, rows * cols), pw,
+        self._call(self.lib.fb_moe_combine_bwd, pg, self._want("moe_combine_backward: ys", ys, rows * cols), pw,
                                                 plan.place.ptr, plan.tokens, plan.k, cols, rows,
                                                 self._want("moe_combine_backward: dys", dys, rows * cols),
-                                                self._want("moe_combine_backward: dweights", dweights, plan.tokens * plan.k)))
+                                                self._want("moe_combine_backward: dweights", dweights, plan.tokens * plan.k))
         return dys, dweights

@@ -54,6 +54,12 @@ cudaError_t allow_dyn_smem(const void* kernel, size_t bytes);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether two arrays of `na` and `nb` elements of `size` bytes share memory (null: none).
+inline bool overlaps(const void* a, uint64_t na, const void* b, uint64_t nb, uint64_t size = 4) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + nb * size && y < x + na * size;
+}
+
 // True when a*b overflows uint64.
 inline bool mul_overflows(uint64_t a, uint64_t b, uint64_t* out) {
   return __builtin_mul_overflow(a, b, out);

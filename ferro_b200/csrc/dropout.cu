@@ -109,10 +109,10 @@ dropout_kernel(const float* x, const float* __restrict__ bias, const float* resi
 // adds the rows in order.
 //
 // Bound by HBM as far as a grid of resident CTAs allows that reads and writes in equal measure: 16384 x
-// 4096 in 96 us, 85 % of the copy rate.  Eight groups are in flight per thread while eight go through the
+// 4096 in 97 us, 84 % of the copy rate.  Seven groups are in flight per thread while seven go through the
 // generator, on two CTAs per SM; four on three, four or five CTAs took 103 to 125 us, without the early
 // loads 109 us at best, a column sum that draws the mask at each load 107 us.
-constexpr int kDropBwdUnroll = 8;      // groups in flight per thread
+constexpr int kDropBwdUnroll = 7;      // groups in flight per thread: 8 spill
 constexpr int kDropBwdPerSm = 2;       // CTAs, by registers
 constexpr uint32_t kDropTile = kDropThreads * 4;
 
@@ -129,11 +129,11 @@ static DropBwdPlan drop_bwd_plan(uint64_t rows, uint64_t cols) {
   const uint64_t target = (uint64_t)device_info().sm_count * kDropBwdPerSm;  // one wave
   p.period = unit;
   double best = 0.0;
-  for (uint64_t m = 1; best < 0.95 && (m <= 16 || unit * m <= kDropTile); ++m) {
+  for (uint64_t m = 1; best < 0.98 && (m <= 16 || unit * m <= kDropTile); ++m) {
     const uint64_t P = unit * m, tiles = (P + kDropTile - 1) / kDropTile;
     if (m > 1 && (tiles > target || P > n / kDropBwdUnroll)) break;
     const double full = (double)P / ((double)tiles * kDropTile);
-    if (full > best + 0.05) {
+    if (full > best + 0.02) {
       best = full;
       p.period = P;
     }
@@ -206,12 +206,21 @@ dropout_bwd_kernel(const float* g, uint64_t n, uint32_t cols, const __grid_const
     float* dp = DX ? dx + at : nullptr;
     uint64_t ctr = M.first() + (at >> 2);
     const uint64_t down = P.period, ctr_down = P.period >> 2;
+    // Columns are summed in blocks of U: the error grows with U + groups / U roundings instead of their number.
+    float sub[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     auto put = [&](float4 v) {
-      v = drop_group(M, ctr, v, acc);
+      v = drop_group(M, ctr, v, sub);
       ctr += ctr_down;
       if (DX) {
         drop_store<VEC>(dp, v);
         dp += down;
+      }
+    };
+    auto fold = [&] {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[j] += sub[j];
+        sub[j] = 0.0f;
       }
     };
     // The next groups' loads are issued before the present ones go through the generator.
@@ -225,6 +234,7 @@ dropout_bwd_kernel(const float* g, uint64_t n, uint32_t cols, const __grid_const
         for (int u = 0; u < U; ++u, gp += down) next[u] = drop_load<VEC>(gp);
 #pragma unroll
         for (int u = 0; u < U; ++u) put(v[u]);
+        fold();
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = next[u];
       }
@@ -234,6 +244,7 @@ dropout_bwd_kernel(const float* g, uint64_t n, uint32_t cols, const __grid_const
         if (u < (int)left) rest[u] = drop_load<VEC>(gp + u * down);
 #pragma unroll
       for (int u = 0; u < U; ++u) put(v[u]);
+      fold();
 #pragma unroll
       for (int u = 0; u < U - 1; ++u)
         if (u < (int)left) put(rest[u]);
@@ -245,6 +256,7 @@ dropout_bwd_kernel(const float* g, uint64_t n, uint32_t cols, const __grid_const
       for (int u = 0; u < U - 1; ++u)
         if (u < (int)left) put(v[u]);
     }
+    fold();
     if (have) {  // the tensor's last group, whole or short
       const float4 w = drop_group(M, M.first() + (last >> 2), drop_load<VEC>(g + last, have), acc);
       if (DX) drop_store<VEC>(dx + last, w, have);
@@ -370,6 +382,8 @@ int fb_dropout_fwd(fb_stream_t stream, const float* x, const float* bias, const 
   if (mul_overflows(rows, cols, &n) || n > (UINT64_MAX >> 3)) return fail(FB_ERR_INVALID_SHAPE, "%s: rows * cols overflows", name);
   if (n == 0) return FB_OK;
   if (!x || !out) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
+  if ((out != x && overlaps(out, n, x, n)) || (out != residual && overlaps(out, n, residual, n)) || overlaps(out, n, bias, cols))
+    return fail(FB_ERR_INVALID_ARG, "%s: out overlaps an input without being x or residual", name);
   if (bias && cols >= (1ull << 31)) return fail(FB_ERR_UNSUPPORTED, "%s: a bias of 2^31 or more elements is not supported", name);
   if (none) return !residual ? fb_fill(stream, out, 0.0f, n) : out == residual ? FB_OK : fb_copy(stream, out, residual, n);
   return run_dropout(stream, name, x, bias, residual, n, cols, m, out);
@@ -395,6 +409,8 @@ int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t c
   if (rows == 0) return dbias ? fb_fill(stream, dbias, 0.0f, cols) : FB_OK;
   if (!g) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (!dx && !dbias) return FB_OK;
+  if ((dx != g && overlaps(dx, n, g, n)) || overlaps(dbias, cols, g, n) || overlaps(dbias, cols, dx, n))
+    return fail(FB_ERR_INVALID_ARG, "%s: dx overlaps g without being it, or dbias overlaps either", name);
   if (none) {
     if (dx)
       if (int rc = fb_fill(stream, dx, 0.0f, n)) return rc;

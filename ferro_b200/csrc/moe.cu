@@ -907,6 +907,9 @@ int fb_moe_gate_fwd(fb_stream_t stream, const float* logits, uint64_t tokens, ui
   if (int rc = gate_check(name, tokens, experts, k)) return rc;
   if (tokens == 0) return FB_OK;
   if (!logits || !weights || !ids) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
+  const uint64_t n = tokens * experts, m = tokens * k;
+  if (overlaps(weights, m, logits, n) || overlaps(ids, 2 * m, logits, n) || overlaps(ids, 2 * m, weights, m))
+    return fail(FB_ERR_INVALID_ARG, "%s: an output overlaps another buffer", name);
   const bool vec = experts % 4 == 0 && aligned16(logits);
   const uint32_t E = (uint32_t)experts, K = (uint32_t)k;
 #define FB_CALL(KL, L, V)                                                                                        \
@@ -934,6 +937,10 @@ int fb_moe_gate_bwd(fb_stream_t stream, const float* dweights, const float* logi
   if (int rc = gate_check(name, tokens, experts, k)) return rc;
   if (tokens == 0) return FB_OK;
   if (!dweights || !weights || !ids || !dlogits || (!renorm && !logits)) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
+  const uint64_t n = tokens * experts, m = tokens * k;
+  if ((!renorm && overlaps(dlogits, n, logits, n)) || overlaps(dlogits, n, weights, m) || overlaps(dlogits, n, dweights, m) ||
+      overlaps(dlogits, n, ids, 2 * m))
+    return fail(FB_ERR_INVALID_ARG, "%s: dlogits overlaps an input", name);
   const bool vec = experts % 4 == 0 && aligned16(dlogits) && (renorm || aligned16(logits));
 #define FB_CALL(L, V, MINE)                                                                                      \
   moe_gate_bwd_kernel<L, V, MINE><<<grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L)), kGateThreads, 0, stream>>>( \
@@ -962,6 +969,9 @@ int fb_moe_sort(fb_stream_t stream, const int64_t* ids, uint64_t n, uint64_t exp
     return fail(FB_ERR_INVALID_SHAPE, "%s: %llu experts, not 1 to %d", name, (unsigned long long)experts, FB_MOE_MAX_EXPERTS);
   if (n > 0x7fffffffull) return fail(FB_ERR_UNSUPPORTED, "%s: 2^31 or more assignments are not supported", name);
   if (!offsets || (n && (!ids || !place))) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
+  if (overlaps(place, n, ids, n, 8) || overlaps(order, n, ids, n, 8) || overlaps(offsets, experts + 1, ids, n, 8) ||
+      overlaps(place, n, order, n, 8) || overlaps(place, n, offsets, experts + 1, 8) || overlaps(order, n, offsets, experts + 1, 8))
+    return fail(FB_ERR_INVALID_ARG, "%s: an output overlaps another buffer", name);
   const uint64_t need = fb_moe_sort_workspace_bytes(n, experts);
   if (need && (!workspace || workspace_bytes < need))
     return fail(FB_ERR_WORKSPACE, "%s: needs %llu bytes of scratch", name, (unsigned long long)need);
@@ -997,7 +1007,8 @@ int fb_moe_dispatch_fwd(fb_stream_t stream, const float* x, const int64_t* place
   if (int rc = rows_check(name, tokens, k, cols, slots)) return rc;
   if (tokens == 0 || cols == 0 || slots == 0) return FB_OK;
   if (!x || !place || !xs) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
-  if (xs == x) return fail(FB_ERR_INVALID_ARG, "%s: xs must not be x", name);
+  if (overlaps(xs, slots * cols, x, tokens * cols) || overlaps(xs, slots * cols, place, 2 * tokens * k))
+    return fail(FB_ERR_INVALID_ARG, "%s: xs must not overlap an input", name);
   const int vec = row_vec(cols, x, xs);
   uint32_t threads;
   const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
@@ -1014,7 +1025,9 @@ static int gather_rows(cudaStream_t stream, const char* name, const float* ys, c
   if (int rc = rows_check(name, tokens, k, cols, slots)) return rc;
   if (tokens == 0 || cols == 0) return FB_OK;
   if ((slots && !ys) || !place || !y) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
-  if (ys == y) return fail(FB_ERR_INVALID_ARG, "%s: the output must not be the input", name);
+  if (overlaps(y, tokens * cols, ys, slots * cols) || overlaps(y, tokens * cols, weights, tokens * k) ||
+      overlaps(y, tokens * cols, place, 2 * tokens * k))
+    return fail(FB_ERR_INVALID_ARG, "%s: the output must not overlap an input", name);
   const int vec = row_vec(cols, ys, y);
   uint32_t threads;
   const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
@@ -1046,7 +1059,11 @@ int fb_moe_combine_bwd(fb_stream_t stream, const float* dy, const float* ys, con
   if (tokens == 0 || (!dys && !dweights)) return FB_OK;
   if (cols == 0) return dweights ? fb_fill(stream, dweights, 0.0f, tokens * k) : FB_OK;
   if (!dy || !weights || !place || (dweights && slots && !ys)) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
-  if (dys == dy || dweights == weights) return fail(FB_ERR_INVALID_ARG, "%s: an output is one of the inputs it must not be", name);
+  const uint64_t n = slots * cols, m = tokens * k;
+  if ((dys != ys && overlaps(dys, n, ys, n)) || overlaps(dys, n, dy, tokens * cols) || overlaps(dys, n, weights, m) ||
+      overlaps(dys, n, place, 2 * m) || overlaps(dweights, m, weights, m) || overlaps(dweights, m, dy, tokens * cols) ||
+      overlaps(dweights, m, ys, n) || overlaps(dweights, m, dys, n) || overlaps(dweights, m, place, 2 * m))
+    return fail(FB_ERR_INVALID_ARG, "%s: an output must not overlap another buffer, but dys may be ys", name);
   const int vec = row_vec(cols, dy, dweights ? ys : dy, dys);
   // A warp per token up to 64 vectors a row, else a CTA with a thread per vector, at most 256.
   const uint64_t vpt = cols / vec;

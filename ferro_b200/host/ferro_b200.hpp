@@ -70,6 +70,19 @@ struct UnaryKind { int code; float p0 = 0.0f, p1 = 0.0f; };    // dispatch.rs:18
 struct BinaryKind { int code; float p0 = 0.0f, p1 = 0.0f; };   // dispatch.rs:68-76
 using AdamWStep = fb_adamw_hparams;                            // dispatch.rs:92-100
 
+// Frequencies of a rotary embedding (rope_plan), with what else stays the same from call to call.
+struct RopePlan {
+  Buf turns;  // i64 [rot_dim / 2]
+  uint64_t rot_dim;
+  int layout;
+  float scale;
+};
+// Assignments sorted by expert (moe_sort_dev).
+struct MoePlan {
+  Buf place, order, offsets;  // i64 [tokens * k], [tokens * k], [experts + 1]
+  uint64_t tokens, k, experts;
+};
+
 class CudaBackend {
  public:
   explicit CudaBackend(int ordinal = 0) : ordinal_(ordinal) {
@@ -306,7 +319,138 @@ class CudaBackend {
   }
   void scalar_increment_dev(DeviceBuffer& t, float beta1, float beta2) { check(fb_scalar_increment(s(), t.f32(), beta1, beta2)); }
 
+  // ---- rotary positions ------------------------------------------------------------------------------------------
+  RopePlan rope_plan(uint64_t rot_dim, double base, int layout, int scaling = FB_ROPE_PLAIN, double factor = 1.0,
+                     double original_len = 0.0, double low = 0.0, double high = 0.0, float scale = 1.0f) {
+    std::vector<int64_t> t(rot_dim / 2);
+    check(fb_rope_turns(rot_dim, base, scaling, factor, original_len, low, high, t.data()));
+    return {alloc_i64_from_host(t), rot_dim, layout, scale};
+  }
+  // x whole and row-major over shape [batch, seq, heads, head_dim]; positions (i64, [seq] or [batch, seq]) or start + 0, 1, ...
+  Buf rope_dev(const DeviceBuffer& x, const std::vector<uint64_t>& shape, const RopePlan& plan, const DeviceBuffer* positions,
+               int64_t start = 0) {
+    return rope(x, shape, plan, positions, start, 0);
+  }
+  Buf rope_backward_dev(const DeviceBuffer& g, const std::vector<uint64_t>& shape, const RopePlan& plan,
+                        const DeviceBuffer* positions, int64_t start = 0) {
+    return rope(g, shape, plan, positions, start, 1);
+  }
+
+  // ---- dropout ---------------------------------------------------------------------------------------------------
+  Buf dropout_dev(const DeviceBuffer& x, const DeviceBuffer* bias, const DeviceBuffer* residual, uint64_t rows, uint64_t cols,
+                  float p, uint64_t seed, uint64_t offset, const DeviceBuffer* counter = nullptr) {
+    want(x, rows * cols);
+    if (bias) want(*bias, cols);
+    if (residual) want(*residual, rows * cols);
+    if (counter) want(*counter, 1, DType::I64);
+    Buf out = alloc_uninit(rows * cols);
+    check(fb_dropout_fwd(s(), x.f32(), bias ? bias->f32() : nullptr, residual ? residual->f32() : nullptr, rows, cols, p, seed,
+                         offset, counter ? counter->i64() : nullptr, out->f32()));
+    return out;
+  }
+  // (dx, dbias) with the mask of the forward's seed, offset and counter.
+  std::pair<Buf, Buf> dropout_backward_dev(const DeviceBuffer& g, uint64_t rows, uint64_t cols, float p, uint64_t seed,
+                                           uint64_t offset, const DeviceBuffer* counter = nullptr) {
+    want(g, rows * cols);
+    if (counter) want(*counter, 1, DType::I64);
+    Buf dx = alloc_uninit(rows * cols), db = alloc_uninit(cols);
+    const uint64_t ws = fb_dropout_bwd_workspace_bytes(rows, cols);
+    check(fb_dropout_bwd(s(), g.f32(), rows, cols, p, seed, offset, counter ? counter->i64() : nullptr, dx->f32(), db->f32(),
+                         scratch(ws), ws));
+    return {std::move(dx), std::move(db)};
+  }
+  void dropout_advance_dev(DeviceBuffer& counter, uint64_t n) {
+    want(counter, 1, DType::I64);
+    check(fb_dropout_advance(s(), counter.i64(), n));
+  }
+
+  // ---- routed experts --------------------------------------------------------------------------------------------
+  // (weights, ids), [tokens, k] each.
+  std::pair<Buf, Buf> moe_gate_dev(const DeviceBuffer& logits, uint64_t tokens, uint64_t experts, uint64_t k, bool renorm) {
+    want(logits, tokens * experts);
+    Buf w = alloc_uninit(tokens * k), ids = alloc_uninit(tokens * k, DType::I64);
+    check(fb_moe_gate_fwd(s(), logits.f32(), tokens, experts, k, renorm ? 1 : 0, w->f32(), ids->i64()));
+    return {std::move(w), std::move(ids)};
+  }
+  Buf moe_gate_backward_dev(const DeviceBuffer& dweights, const DeviceBuffer& logits, const DeviceBuffer& weights,
+                            const DeviceBuffer& ids, uint64_t tokens, uint64_t experts, uint64_t k, bool renorm) {
+    want(dweights, tokens * k);
+    want(logits, tokens * experts);
+    want(weights, tokens * k);
+    want(ids, tokens * k, DType::I64);
+    Buf dl = alloc_uninit(tokens * experts);
+    check(fb_moe_gate_bwd(s(), dweights.f32(), logits.f32(), weights.f32(), ids.i64(), tokens, experts, k, renorm ? 1 : 0, dl->f32()));
+    return dl;
+  }
+  MoePlan moe_sort_dev(const DeviceBuffer& ids, uint64_t tokens, uint64_t k, uint64_t experts) {
+    const uint64_t n = tokens * k;
+    want(ids, n, DType::I64);
+    MoePlan p{alloc_uninit(n, DType::I64), alloc_uninit(n, DType::I64), alloc_uninit(experts + 1, DType::I64), tokens, k, experts};
+    const uint64_t ws = fb_moe_sort_workspace_bytes(n, experts);
+    check(fb_moe_sort(s(), ids.i64(), n, experts, p.place->i64(), p.order->i64(), p.offsets->i64(), nullptr, scratch(ws), ws));
+    return p;
+  }
+  // Expert-sorted rows of tokens * k; those behind the last assignment are left uninitialised.
+  Buf moe_dispatch_dev(const DeviceBuffer& x, const MoePlan& p, uint64_t cols) {
+    want(x, p.tokens * cols);
+    Buf xs = alloc_uninit(p.tokens * p.k * cols);
+    check(fb_moe_dispatch_fwd(s(), x.f32(), p.place->i64(), p.tokens, p.k, cols, xs->f32(), p.tokens * p.k));
+    return xs;
+  }
+  Buf moe_dispatch_backward_dev(const DeviceBuffer& g, const MoePlan& p, uint64_t cols) {
+    want(g, p.tokens * p.k * cols);
+    Buf dx = alloc_uninit(p.tokens * cols);
+    check(fb_moe_dispatch_bwd(s(), g.f32(), p.place->i64(), p.tokens, p.k, cols, p.tokens * p.k, dx->f32()));
+    return dx;
+  }
+  Buf moe_combine_dev(const DeviceBuffer& ys, const DeviceBuffer& weights, const MoePlan& p, uint64_t cols) {
+    want(ys, p.tokens * p.k * cols);
+    want(weights, p.tokens * p.k);
+    Buf y = alloc_uninit(p.tokens * cols);
+    check(fb_moe_combine_fwd(s(), ys.f32(), weights.f32(), p.place->i64(), p.tokens, p.k, cols, p.tokens * p.k, y->f32()));
+    return y;
+  }
+  // (dys, dweights)
+  std::pair<Buf, Buf> moe_combine_backward_dev(const DeviceBuffer& g, const DeviceBuffer& ys, const DeviceBuffer& weights,
+                                               const MoePlan& p, uint64_t cols) {
+    want(g, p.tokens * cols);
+    want(ys, p.tokens * p.k * cols);
+    want(weights, p.tokens * p.k);
+    Buf dys = alloc_uninit(p.tokens * p.k * cols), dw = alloc_uninit(p.tokens * p.k);
+    check(fb_moe_combine_bwd(s(), g.f32(), ys.f32(), weights.f32(), p.place->i64(), p.tokens, p.k, cols, p.tokens * p.k, dys->f32(), dw->f32()));
+    return {std::move(dys), std::move(dw)};
+  }
+
  private:
+  static void want(const DeviceBuffer& b, uint64_t n, DType dt = DType::F32) {
+    if (b.dtype() != dt) throw Unsupported(dt == DType::F32 ? "an f32 buffer is needed" : "an i64 buffer is needed");
+    if (b.len() != n) throw InvalidShape("buffer has " + std::to_string(b.len()) + " elements, expected " + std::to_string(n));
+  }
+  Buf rope(const DeviceBuffer& x, const std::vector<uint64_t>& shape, const RopePlan& plan, const DeviceBuffer* positions,
+           int64_t start, int inverse) {
+    if (shape.size() != 4) throw InvalidShape("rope: the shape is not [batch, seq, heads, head_dim]");
+    want(x, numel(shape));
+    fb_view v = {};
+    v.ptr = x.f32();
+    v.len = x.len();
+    v.rank = 4;
+    int64_t st = 1;
+    for (int d = 3; d >= 0; --d) {
+      v.shape[d] = shape[d];
+      v.strides[d] = st;
+      st *= (int64_t)shape[d];
+    }
+    uint64_t rows = 1;
+    if (positions) {
+      if (positions->len() != shape[1] && positions->len() != shape[0] * shape[1]) throw InvalidShape("rope: wrong number of positions");
+      want(*positions, positions->len(), DType::I64);
+      rows = positions->len() == shape[1] ? 1 : shape[0];
+    }
+    Buf out = alloc_uninit(x.len());
+    check(fb_rope(s(), &v, positions ? positions->i64() : nullptr, rows, start, plan.turns->i64(), plan.rot_dim, plan.layout,
+                  plan.scale, inverse, out->f32(), out->len(), nullptr, 0));
+    return out;
+  }
   fb_stream_t s() const { return reinterpret_cast<fb_stream_t>(stream_); }
   static uint64_t numel(const std::vector<uint64_t>& shape) {
     uint64_t n = 1;

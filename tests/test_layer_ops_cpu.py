@@ -113,11 +113,18 @@ def test_dropout_refusals(lib):
     says(lib, lib.fb_dropout_fwd(None, None, None, None, 2, 4, 0.1, 1, 0, None, P), 2, "null")
     says(lib, lib.fb_dropout_fwd(None, P, None, None, 2, 4, 0.1, 1, 0, None, None), 2, "null")
     says(lib, lib.fb_dropout_bwd(None, None, 2, 4, 0.1, 1, 0, None, P, None, None, 0), 2, "null")
-    says(lib, lib.fb_dropout_fwd(None, P, P, None, 1, 1 << 31, 0.1, 1, 0, None, P), 4, "bias")
+    says(lib, lib.fb_dropout_fwd(None, P, P - 64, None, 1, 1 << 31, 0.1, 1, 0, None, P + (1 << 40)), 4, "bias")
+    # outputs that overlap an input without being it
+    says(lib, lib.fb_dropout_fwd(None, P, None, None, 2, 4, 0.1, 1, 0, None, P + 4), 2, "overlaps")
+    says(lib, lib.fb_dropout_fwd(None, P, None, 2 * P, 2, 4, 0.1, 1, 0, None, 2 * P - 4), 2, "overlaps")
+    says(lib, lib.fb_dropout_fwd(None, P, 2 * P, None, 2, 4, 0.1, 1, 0, None, 2 * P + 8), 2, "overlaps")
+    says(lib, lib.fb_dropout_bwd(None, P, 2, 4, 0.1, 1, 0, None, P + 16, None, None, 0), 2, "overlaps")
+    says(lib, lib.fb_dropout_bwd(None, P, 2, 4, 0.1, 1, 0, None, 2 * P, P + 16, None, 0), 2, "overlaps")
+    says(lib, lib.fb_dropout_bwd(None, P, 2, 4, 0.1, 1, 0, None, 2 * P, 2 * P, None, 0), 2, "overlaps")
     need = lib.fb_dropout_bwd_workspace_bytes(100000, 64)
     assert need > 0
-    says(lib, lib.fb_dropout_bwd(None, P, 100000, 64, 0.1, 1, 0, None, P, P, None, 0), 5, "scratch")
-    says(lib, lib.fb_dropout_bwd(None, P, 100000, 64, 0.1, 1, 0, None, P, P, P, need - 1), 5, "scratch")
+    says(lib, lib.fb_dropout_bwd(None, 1 << 40, 100000, 64, 0.1, 1, 0, None, 1 << 40, P, None, 0), 5, "scratch")
+    says(lib, lib.fb_dropout_bwd(None, 1 << 40, 100000, 64, 0.1, 1, 0, None, 1 << 40, P, P, need - 1), 5, "scratch")
     says(lib, lib.fb_dropout_advance(None, None, 1), 2, "null")
     assert lib.fb_dropout_fwd(None, None, None, None, 0, 4, 0.1, 1, 0, None, None) == 0
     assert lib.fb_dropout_bwd(None, P, 4, 0, 0.1, 1, 0, None, P, P, None, 0) == 0
@@ -139,9 +146,15 @@ def test_expert_refusals(lib):
     says(lib, lib.fb_moe_sort(None, None, 8, 4, P, P, P, None, None, 0), 2, "null")
     says(lib, lib.fb_moe_sort(None, P, 8, 4, None, P, P, None, None, 0), 2, "null")
     says(lib, lib.fb_moe_sort(None, P, 8, 4, P, P, None, None, None, 0), 2, "null")
+    for a in ([P + 8, 2 * P, 3 * P], [P, P, 3 * P], [2 * P, 2 * P + 8, 3 * P], [2 * P, 3 * P, 3 * P - 8], [2 * P, 3 * P, P + 56]):
+        says(lib, lib.fb_moe_sort(None, P, 8, 4, a[0], a[1], a[2], None, None, 0), 2, "overlaps")
+    for a in ([P + 4, 3 * P], [2 * P, P], [2 * P, 2 * P + 12]):
+        says(lib, lib.fb_moe_gate_fwd(None, P, 2, 4, 2, 1, a[0], a[1]), 2, "overlaps")
+    for a in (P, 2 * P + 4, 3 * P, 4 * P + 24):
+        says(lib, lib.fb_moe_gate_bwd(None, P, 2 * P, 3 * P, 4 * P, 2, 4, 2, 0, a), 2, "overlaps")
     need = lib.fb_moe_sort_workspace_bytes(1 << 20, 64)
     assert need > 0 and lib.fb_moe_sort_workspace_bytes(100, 64) == 0
-    says(lib, lib.fb_moe_sort(None, P, 1 << 20, 64, P, P, P, None, P, need - 1), 5, "scratch")
+    says(lib, lib.fb_moe_sort(None, 1 << 32, 1 << 20, 64, 1 << 33, 1 << 34, 1 << 35, None, P, need - 1), 5, "scratch")
     for k in (0, 33):
         says(lib, lib.fb_moe_dispatch_fwd(None, P, P, 2, k, 4, 2 * P, 8), 1, "k ")
         says(lib, lib.fb_moe_dispatch_bwd(None, P, P, 2, k, 4, 8, 2 * P), 1, "k ")
@@ -150,12 +163,20 @@ def test_expert_refusals(lib):
     says(lib, lib.fb_moe_dispatch_fwd(None, P, P, 1 << 62, 2, 4, 2 * P, 8), 1, "overflow")
     says(lib, lib.fb_moe_dispatch_fwd(None, P, P, 2, 2, 4, 2 * P, 1 << 62), 1, "overflow")
     says(lib, lib.fb_moe_dispatch_fwd(None, P, None, 2, 2, 4, 2 * P, 8), 2, "null")
-    says(lib, lib.fb_moe_dispatch_fwd(None, P, P, 2, 2, 4, P, 8), 2, "must not")
+    says(lib, lib.fb_moe_dispatch_fwd(None, P, 3 * P, 2, 2, 4, P, 8), 2, "must not")
     says(lib, lib.fb_moe_dispatch_bwd(None, None, P, 2, 2, 4, 8, P), 2, "null")
-    says(lib, lib.fb_moe_dispatch_bwd(None, P, P, 2, 2, 4, 8, P), 2, "must not")
+    says(lib, lib.fb_moe_dispatch_bwd(None, P, 3 * P, 2, 2, 4, 8, P + 64), 2, "must not")
     says(lib, lib.fb_moe_combine_fwd(None, P, None, P, 2, 2, 4, 8, 2 * P), 2, "null")
     says(lib, lib.fb_moe_combine_bwd(None, P, None, P, P, 2, 2, 4, 8, 2 * P, 3 * P), 2, "null")
-    says(lib, lib.fb_moe_combine_bwd(None, P, 2 * P, P, P, 2, 2, 4, 8, P, 3 * P), 2, "must not")
+    says(lib, lib.fb_moe_dispatch_fwd(None, P, 3 * P, 2, 2, 4, P + 28, 8), 2, "must not")
+    says(lib, lib.fb_moe_dispatch_fwd(None, P, 3 * P, 2, 2, 4, 3 * P, 8), 2, "must not")
+    for y in (P + 124, 2 * P, 3 * P):
+        says(lib, lib.fb_moe_combine_fwd(None, P, 2 * P, 3 * P, 2, 2, 4, 8, y), 2, "must not")
+    # dy, ys, weights, place -> dys, dweights: dys may be ys and nothing else
+    for a in ([P, 6 * P], [2 * P + 4, 6 * P], [3 * P, 6 * P], [4 * P, 6 * P], [5 * P, P], [5 * P, 2 * P], [5 * P, 3 * P], [5 * P, 4 * P],
+              [5 * P, 5 * P], [2 * P, 2 * P + 16]):
+        says(lib, lib.fb_moe_combine_bwd(None, P, 2 * P, 3 * P, 4 * P, 2, 2, 4, 8, a[0], a[1]), 2, "must not")
+    says(lib, lib.fb_moe_dispatch_fwd(None, P, 3 * P, 2, 2, 1 << 31, 2 * P, 8), 4, "2^31")
     # nothing to do
     assert lib.fb_moe_gate_fwd(None, None, 0, 4, 2, 1, None, None) == 0
     assert lib.fb_moe_gate_bwd(None, None, None, None, None, 0, 4, 2, 0, None) == 0
