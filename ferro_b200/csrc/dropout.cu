@@ -36,6 +36,8 @@ template <bool VEC, int BIAS, bool RES>
 __global__ void __launch_bounds__(kDropThreads)
 dropout_kernel(const float* x, const float* __restrict__ bias, const float* residual, uint64_t n, uint32_t cols,
                FastDiv d_cols, DropMask M, float* out) {
+  pdl_wait();
+  pdl_trigger();
   const uint64_t groups = (n + 3) / 4;
   const uint64_t first = M.first();
   for (uint64_t base = (uint64_t)blockIdx.x * kDropThreads * kDropUnroll; base < groups;
@@ -185,6 +187,7 @@ template <bool VEC, bool DX>
 __global__ void __launch_bounds__(kDropThreads, kDropBwdPerSm)
 dropout_bwd_kernel(const float* g, uint64_t n, uint32_t cols, const __grid_constant__ DropBwdPlan P, DropMask M,
                    float* dx, float* __restrict__ sums) {
+  pdl_wait();
   pdl_trigger();
   __shared__ __align__(16) float sm[kDropTile];
   __shared__ float part[kDropThreads];
@@ -322,6 +325,8 @@ dropout_bias_kernel(const float* __restrict__ part, uint32_t rows, uint64_t cols
 }
 
 __global__ void dropout_advance_kernel(int64_t* counter, uint64_t n) {
+  pdl_wait();
+  pdl_trigger();
   if (threadIdx.x == 0) counter[0] = (int64_t)((uint64_t)counter[0] + n);
 }
 
@@ -339,31 +344,27 @@ static int make_mask(const char* name, float p, uint64_t seed, uint64_t offset, 
 }
 
 template <bool VEC, int BIAS>
-static void drop_launch(cudaStream_t s, unsigned grid, const float* x, const float* bias, const float* residual,
+static int drop_launch(cudaStream_t s, unsigned grid, const float* x, const float* bias, const float* residual,
                         uint64_t n, uint64_t cols, const DropMask& m, float* out) {
   const uint32_t c32 = (uint32_t)cols;
   const FastDiv d = make_fastdiv(BIAS == DROP_NO_BIAS ? 1 : c32);
-  if (residual) dropout_kernel<VEC, BIAS, true><<<grid, kDropThreads, 0, s>>>(x, bias, residual, n, c32, d, m, out);
-  else dropout_kernel<VEC, BIAS, false><<<grid, kDropThreads, 0, s>>>(x, bias, residual, n, c32, d, m, out);
+  if (residual) FB_CUDA(launch_pdl(dropout_kernel<VEC, BIAS, true>, dim3(grid), dim3(kDropThreads), 0, s, x, bias, residual, n, c32, d, m, out));
+  else FB_CUDA(launch_pdl(dropout_kernel<VEC, BIAS, false>, dim3(grid), dim3(kDropThreads), 0, s, x, bias, residual, n, c32, d, m, out));
+  FB_LAUNCHED("fb_dropout");
+  return FB_OK;
 }
 
-static int run_dropout(cudaStream_t s, const char* name, const float* x, const float* bias, const float* residual,
+static int run_dropout(cudaStream_t s, const float* x, const float* bias, const float* residual,
                        uint64_t n, uint64_t cols, const DropMask& m, float* out) {
   const bool vec = aligned16(x) && aligned16(out) && (!residual || aligned16(residual));
   const uint64_t per_cta = (uint64_t)kDropThreads * kDropUnroll;
   const unsigned grid = grid_full(((n + 3) / 4 + per_cta - 1) / per_cta);
-  if (!bias) {
-    if (vec) drop_launch<true, DROP_NO_BIAS>(s, grid, x, bias, residual, n, cols, m, out);
-    else drop_launch<false, DROP_NO_BIAS>(s, grid, x, bias, residual, n, cols, m, out);
-  } else if (vec && cols % 4 == 0 && aligned16(bias)) {
-    drop_launch<true, DROP_BIAS_VEC>(s, grid, x, bias, residual, n, cols, m, out);
-  } else if (vec) {
-    drop_launch<true, DROP_BIAS_SCALAR>(s, grid, x, bias, residual, n, cols, m, out);
-  } else {
-    drop_launch<false, DROP_BIAS_SCALAR>(s, grid, x, bias, residual, n, cols, m, out);
-  }
-  FB_LAUNCHED(name);
-  return FB_OK;
+  if (!bias)
+    return vec ? drop_launch<true, DROP_NO_BIAS>(s, grid, x, bias, residual, n, cols, m, out)
+               : drop_launch<false, DROP_NO_BIAS>(s, grid, x, bias, residual, n, cols, m, out);
+  if (vec && cols % 4 == 0 && aligned16(bias)) return drop_launch<true, DROP_BIAS_VEC>(s, grid, x, bias, residual, n, cols, m, out);
+  return vec ? drop_launch<true, DROP_BIAS_SCALAR>(s, grid, x, bias, residual, n, cols, m, out)
+             : drop_launch<false, DROP_BIAS_SCALAR>(s, grid, x, bias, residual, n, cols, m, out);
 }
 
 }  // namespace fb
@@ -386,7 +387,7 @@ int fb_dropout_fwd(fb_stream_t stream, const float* x, const float* bias, const 
     return fail(FB_ERR_INVALID_ARG, "%s: out overlaps an input without being x or residual", name);
   if (bias && cols >= (1ull << 31)) return fail(FB_ERR_UNSUPPORTED, "%s: a bias of 2^31 or more elements is not supported", name);
   if (none) return !residual ? fb_fill(stream, out, 0.0f, n) : out == residual ? FB_OK : fb_copy(stream, out, residual, n);
-  return run_dropout(stream, name, x, bias, residual, n, cols, m, out);
+  return run_dropout(stream, x, bias, residual, n, cols, m, out);
 }
 
 uint64_t fb_dropout_bwd_workspace_bytes(uint64_t rows, uint64_t cols) {
@@ -416,7 +417,7 @@ int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t c
       if (int rc = fb_fill(stream, dx, 0.0f, n)) return rc;
     return dbias ? fb_fill(stream, dbias, 0.0f, cols) : FB_OK;
   }
-  if (!dbias) return run_dropout(stream, name, g, nullptr, nullptr, n, cols, m, dx);
+  if (!dbias) return run_dropout(stream, g, nullptr, nullptr, n, cols, m, dx);
   if (cols >= (1ull << 31)) return fail(FB_ERR_UNSUPPORTED, "%s: a bias of 2^31 or more elements is not supported", name);
   const DropBwdPlan plan = drop_bwd_plan(rows, cols);
   const uint64_t need = fb_dropout_bwd_workspace_bytes(rows, cols);
@@ -425,10 +426,10 @@ int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t c
   float* sums = need ? static_cast<float*>(workspace) : dbias;
   const unsigned grid = plan.tiles * plan.slabs;
   const bool vec = aligned16(g) && (!dx || aligned16(dx));
-  if (vec && dx) dropout_bwd_kernel<true, true><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
-  else if (vec) dropout_bwd_kernel<true, false><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
-  else if (dx) dropout_bwd_kernel<false, true><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
-  else dropout_bwd_kernel<false, false><<<grid, kDropThreads, 0, stream>>>(g, n, (uint32_t)cols, plan, m, dx, sums);
+  if (vec && dx) FB_CUDA(launch_pdl(dropout_bwd_kernel<true, true>, dim3(grid), dim3(kDropThreads), 0, stream, g, n, (uint32_t)cols, plan, m, dx, sums));
+  else if (vec) FB_CUDA(launch_pdl(dropout_bwd_kernel<true, false>, dim3(grid), dim3(kDropThreads), 0, stream, g, n, (uint32_t)cols, plan, m, dx, sums));
+  else if (dx) FB_CUDA(launch_pdl(dropout_bwd_kernel<false, true>, dim3(grid), dim3(kDropThreads), 0, stream, g, n, (uint32_t)cols, plan, m, dx, sums));
+  else FB_CUDA(launch_pdl(dropout_bwd_kernel<false, false>, dim3(grid), dim3(kDropThreads), 0, stream, g, n, (uint32_t)cols, plan, m, dx, sums));
   FB_LAUNCHED(name);
   if (need) {
     FB_CUDA(launch_pdl(dropout_bias_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, stream, (const float*)sums,
@@ -440,7 +441,7 @@ int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t c
 
 int fb_dropout_advance(fb_stream_t stream, int64_t* counter, uint64_t n) {
   if (!counter) return fail(FB_ERR_INVALID_ARG, "fb_dropout_advance: null counter");
-  dropout_advance_kernel<<<1, 32, 0, stream>>>(counter, n);
+  FB_CUDA(launch_pdl(dropout_advance_kernel, dim3(1), dim3(32), 0, stream, counter, n));
   FB_LAUNCHED("fb_dropout_advance");
   return FB_OK;
 }

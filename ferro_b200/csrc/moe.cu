@@ -175,6 +175,8 @@ moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t 
   static_assert(KL <= L, "lane l of a token reports choice l");
   constexpr uint32_t kIds = L * V, kKept = ~(kIds - 1);  // a power of two
   constexpr int kTokens = 32 / L;                        // per warp
+  pdl_wait();
+  pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, g = lane / L;
   const uint64_t step = (uint64_t)gridDim.x * kGateWarps * kTokens;
   for (uint64_t t0 = ((uint64_t)blockIdx.x * kGateWarps + warp) * kTokens; t0 < tokens; t0 += step) {
@@ -260,6 +262,8 @@ template <int NPL>
 __global__ void __launch_bounds__(kGateThreads)
 moe_gate_fwd_many_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t experts, uint32_t k, bool renorm,
                          float* __restrict__ weights, int64_t* __restrict__ ids) {
+  pdl_wait();
+  pdl_trigger();
   constexpr uint32_t kIds = 32 * NPL, kKept = ~(kIds - 1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (uint64_t t = (uint64_t)blockIdx.x * kGateWarps + warp; t < tokens; t += (uint64_t)gridDim.x * kGateWarps) {
@@ -328,6 +332,8 @@ __global__ void __launch_bounds__(kGateThreads)
 moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict__ logits, const float* __restrict__ weights,
                     const int64_t* __restrict__ ids, uint64_t tokens, uint32_t experts, uint32_t k, bool renorm, bool vec,
                     float* __restrict__ dlogits) {
+  pdl_wait();
+  pdl_trigger();
   constexpr int kTokens = 32 / L;  // MINE choices a lane
   __shared__ __align__(16) float rows[kGateThreads / L][L * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % L, g = lane / L;
@@ -437,6 +443,7 @@ __device__ __forceinline__ uint32_t lanes_alike(uint32_t id, int bits) {
 template <int R>
 __global__ void __launch_bounds__(kSortThreads)
 moe_count_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, uint32_t* __restrict__ counts) {
+  pdl_wait();  // before the trigger: moe_place_kernel relies on what this kernel waited for
   pdl_trigger();
   extern __shared__ uint32_t hist[];
   const uint32_t base = blockIdx.x * (kSortThreads * R);
@@ -499,8 +506,10 @@ moe_place_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
   uint32_t* before = total + experts;   // [experts] in the chunks before this one
   uint32_t* hist = before + experts;    // [warps][stride]
   __shared__ uint32_t wsum[32];
-  // The ids are older than the kernel before this one (moe_count_kernel only reads them, and started
-  // after whatever wrote them had ended): they may be read before pdl_wait.
+  // Behind moe_count_kernel (or moe_scan_kernel) the ids may be read before pdl_wait: those kernels only
+  // let this one start after they had waited for whatever wrote them.
+  if (mode == SORT_ALONE) pdl_wait();
+  pdl_trigger();
   const uint32_t base = blockIdx.x * (blockDim.x * R) + warp * 32 * R + lane;
   uint32_t id[R], rank[R];
 #pragma unroll
@@ -666,6 +675,8 @@ template <int VEC, int KU>
 __global__ void __launch_bounds__(kRowThreads, KU == 8 ? 4 : 5)
 moe_scatter_kernel(const float* __restrict__ x, const int64_t* __restrict__ place, const __grid_constant__ RowMap M,
                    float* __restrict__ xs) {
+  pdl_wait();
+  pdl_trigger();
   for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
     uint64_t t;
     uint32_t vec, end;
@@ -692,6 +703,8 @@ template <int VEC, int KU, bool WEIGHTED>
 __global__ void __launch_bounds__(kRowThreads, KU == 8 ? 3 : 5)
 moe_gather_kernel(const float* __restrict__ ys, const float* __restrict__ weights, const int64_t* __restrict__ place,
                   const __grid_constant__ RowMap M, float* __restrict__ y) {
+  pdl_wait();
+  pdl_trigger();
   for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
     uint64_t t;
     uint32_t vec, end;
@@ -733,6 +746,8 @@ __global__ void __launch_bounds__(kRowThreads, KU == 8 ? 2 : 3)
 moe_combine_bwd_kernel(const float* __restrict__ dy, const float* ys, const float* __restrict__ weights,
                        const int64_t* __restrict__ place, uint64_t tokens, uint32_t k, uint64_t cols, uint64_t slots,
                        float* dys, float* __restrict__ dweights) {
+  pdl_wait();
+  pdl_trigger();
   __shared__ float part[kRowThreads / 32][KU];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const uint64_t first = WARP ? (uint64_t)blockIdx.x * warps + warp : blockIdx.x;
@@ -913,13 +928,13 @@ int fb_moe_gate_fwd(fb_stream_t stream, const float* logits, uint64_t tokens, ui
   const bool vec = experts % 4 == 0 && aligned16(logits);
   const uint32_t E = (uint32_t)experts, K = (uint32_t)k;
 #define FB_CALL(KL, L, V)                                                                                        \
-  moe_gate_fwd_kernel<KL, L, V><<<grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L)), kGateThreads, 0, stream>>>( \
-      logits, tokens, E, K, renorm != 0, vec, weights, ids)
+  FB_CUDA(launch_pdl(moe_gate_fwd_kernel<KL, L, V>, dim3(grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L))), dim3(kGateThreads), 0, stream, \
+      logits, tokens, E, K, renorm != 0, vec, weights, ids))
 #define FB_CALL2(L, V) FB_CALL(2, L, V)
 #define FB_CALL8(L, V) FB_CALL(8, L, V)
 #define FB_MANY(NPL)                                                                                             \
-  moe_gate_fwd_many_kernel<NPL><<<grid_full((tokens + kGateWarps - 1) / kGateWarps), kGateThreads, 0, stream>>>( \
-      logits, tokens, E, K, renorm != 0, weights, ids)
+  FB_CUDA(launch_pdl(moe_gate_fwd_many_kernel<NPL>, dim3(grid_full((tokens + kGateWarps - 1) / kGateWarps)), dim3(kGateThreads), 0, stream, \
+      logits, tokens, E, K, renorm != 0, weights, ids))
   if (k <= 2) FB_GATE_ROWS(experts, FB_CALL2);
   else if (k <= 8) FB_GATE_ROWS(experts, FB_CALL8);
   else FB_GATE_WARP(experts, FB_MANY);
@@ -943,8 +958,8 @@ int fb_moe_gate_bwd(fb_stream_t stream, const float* dweights, const float* logi
     return fail(FB_ERR_INVALID_ARG, "%s: dlogits overlaps an input", name);
   const bool vec = experts % 4 == 0 && aligned16(dlogits) && (renorm || aligned16(logits));
 #define FB_CALL(L, V, MINE)                                                                                      \
-  moe_gate_bwd_kernel<L, V, MINE><<<grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L)), kGateThreads, 0, stream>>>( \
-      dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, renorm != 0, vec, dlogits)
+  FB_CUDA(launch_pdl(moe_gate_bwd_kernel<L, V, MINE>, dim3(grid_full((tokens + kGateThreads / L - 1) / (kGateThreads / L))), dim3(kGateThreads), 0, stream, \
+      dweights, logits, weights, ids, tokens, (uint32_t)experts, (uint32_t)k, renorm != 0, vec, dlogits))
 #define FB_CALL1(L, V) FB_CALL(L, V, 1)
 #define FB_CALL_ALL(L, V) FB_CALL(L, V, (FB_MOE_MAX_K / L))
   if (k <= 8) FB_GATE_ROWS(experts, FB_CALL1);
@@ -983,13 +998,13 @@ int fb_moe_sort(fb_stream_t stream, const int64_t* ids, uint64_t n, uint64_t exp
   uint32_t* counts = static_cast<uint32_t*>(workspace);
   uint32_t* totals = counts + (uint64_t)p.chunks * E;
   if (p.mode == SORT_ALONE) {
-    if (one) moe_place_kernel<1><<<1, p.threads, smem, stream>>>(ids, n32, E, 1, p.mode, nullptr, nullptr, place, order, offsets, bad_index);
-    else moe_place_kernel<kSortRounds><<<1, p.threads, smem, stream>>>(ids, n32, E, 1, p.mode, nullptr, nullptr, place, order, offsets, bad_index);
+    if (one) FB_CUDA(launch_pdl(moe_place_kernel<1>, dim3(1), dim3(p.threads), smem, stream, ids, n32, E, 1, p.mode, nullptr, nullptr, place, order, offsets, bad_index));
+    else FB_CUDA(launch_pdl(moe_place_kernel<kSortRounds>, dim3(1), dim3(p.threads), smem, stream, ids, n32, E, 1, p.mode, nullptr, nullptr, place, order, offsets, bad_index));
     FB_LAUNCHED(name);
     return FB_OK;
   }
-  if (one) moe_count_kernel<1><<<p.chunks, kSortThreads, E * sizeof(uint32_t), stream>>>(ids, n32, E, counts);
-  else moe_count_kernel<kSortRounds><<<p.chunks, kSortThreads, E * sizeof(uint32_t), stream>>>(ids, n32, E, counts);
+  if (one) FB_CUDA(launch_pdl(moe_count_kernel<1>, dim3(p.chunks), dim3(kSortThreads), E * sizeof(uint32_t), stream, ids, n32, E, counts));
+  else FB_CUDA(launch_pdl(moe_count_kernel<kSortRounds>, dim3(p.chunks), dim3(kSortThreads), E * sizeof(uint32_t), stream, ids, n32, E, counts));
   FB_LAUNCHED(name);
   if (p.mode == SORT_SCANNED) {
     FB_CUDA(launch_pdl(moe_scan_kernel, dim3((E + 31) / 32), dim3(1024), 0, stream, counts, p.chunks, E, totals));
@@ -1013,7 +1028,7 @@ int fb_moe_dispatch_fwd(fb_stream_t stream, const float* x, const int64_t* place
   uint32_t threads;
   const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
   const unsigned grid = grid_full(m.blocks);
-#define FB_CALL(VEC, KU) moe_scatter_kernel<VEC, KU><<<grid, threads, 0, stream>>>(x, place, m, xs)
+#define FB_CALL(VEC, KU) FB_CUDA(launch_pdl(moe_scatter_kernel<VEC, KU>, dim3(grid), dim3(threads), 0, stream, x, place, m, xs))
   FB_ROW_DISPATCH(vec, k, true, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
@@ -1033,8 +1048,8 @@ static int gather_rows(cudaStream_t stream, const char* name, const float* ys, c
   const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
   const unsigned grid = grid_full(m.blocks);
 #define FB_CALL(VEC, KU)                                                                                            \
-  if (weights) moe_gather_kernel<VEC, KU, true><<<grid, threads, 0, stream>>>(ys, weights, place, m, y);            \
-  else moe_gather_kernel<VEC, KU, false><<<grid, threads, 0, stream>>>(ys, weights, place, m, y)
+  if (weights) FB_CUDA(launch_pdl(moe_gather_kernel<VEC, KU, true>, dim3(grid), dim3(threads), 0, stream, ys, weights, place, m, y));            \
+  else FB_CUDA(launch_pdl(moe_gather_kernel<VEC, KU, false>, dim3(grid), dim3(threads), 0, stream, ys, weights, place, m, y))
   FB_ROW_DISPATCH(vec, k, few_tokens(tokens), FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
@@ -1072,8 +1087,8 @@ int fb_moe_combine_bwd(fb_stream_t stream, const float* dy, const float* ys, con
   const unsigned grid = grid_full(by_warp ? (tokens + kRowThreads / 32 - 1) / (kRowThreads / 32) : tokens);
   const uint32_t k32 = (uint32_t)k;
 #define FB_CALL(VEC, KU)                                                                                                              \
-  if (by_warp) moe_combine_bwd_kernel<VEC, KU, true><<<grid, threads, 0, stream>>>(dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights); \
-  else moe_combine_bwd_kernel<VEC, KU, false><<<grid, threads, 0, stream>>>(dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights)
+  if (by_warp) FB_CUDA(launch_pdl(moe_combine_bwd_kernel<VEC, KU, true>, dim3(grid), dim3(threads), 0, stream, dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights)); \
+  else FB_CUDA(launch_pdl(moe_combine_bwd_kernel<VEC, KU, false>, dim3(grid), dim3(threads), 0, stream, dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights))
   FB_ROW_DISPATCH(vec, k, true, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);

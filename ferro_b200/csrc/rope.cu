@@ -93,6 +93,8 @@ template <int VEC, int LAYOUT, int HPT>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs A) {
   constexpr bool kTwo = LAYOUT == FB_ROPE_HALF || VEC == 1;  // two vectors per group
   constexpr int kPairs = LAYOUT == FB_ROPE_HALF ? VEC : (VEC + 1) / 2;
+  pdl_wait();
+  pdl_trigger();
   for (uint64_t blk = blockIdx.x; blk < A.blocks; blk += gridDim.x) {
     uint32_t token, rem;
     if (A.bpt == 1) {
@@ -184,10 +186,10 @@ static int rope_launch(cudaStream_t stream, RopeArgs& A, bool in_place, uint32_t
   A.d_seq = make_fastdiv(A.seq);
   A.blocks = (uint64_t)((A.tokens + A.tpb - 1) / A.tpb) * A.bpt;
   const unsigned grid = grid_full(A.blocks);
-  if (hpt == 1) rope_kernel<VEC, LAYOUT, 1><<<grid, kRopeThreads, 0, stream>>>(A);
-  else if (hpt == 2) rope_kernel<VEC, LAYOUT, 2><<<grid, kRopeThreads, 0, stream>>>(A);
-  else if (hpt == 4) rope_kernel<VEC, LAYOUT, 4><<<grid, kRopeThreads, 0, stream>>>(A);
-  else if constexpr (VEC < 4) rope_kernel<VEC, LAYOUT, 8><<<grid, kRopeThreads, 0, stream>>>(A);
+  if (hpt == 1) FB_CUDA(launch_pdl(rope_kernel<VEC, LAYOUT, 1>, dim3(grid), dim3(kRopeThreads), 0, stream, A));
+  else if (hpt == 2) FB_CUDA(launch_pdl(rope_kernel<VEC, LAYOUT, 2>, dim3(grid), dim3(kRopeThreads), 0, stream, A));
+  else if (hpt == 4) FB_CUDA(launch_pdl(rope_kernel<VEC, LAYOUT, 4>, dim3(grid), dim3(kRopeThreads), 0, stream, A));
+  else if constexpr (VEC < 4) FB_CUDA(launch_pdl(rope_kernel<VEC, LAYOUT, 8>, dim3(grid), dim3(kRopeThreads), 0, stream, A));
   FB_LAUNCHED("fb_rope");
   return FB_OK;
 }
