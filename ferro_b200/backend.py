@@ -10,6 +10,7 @@ buffer.  torch supplies device memory and the stream, nothing else: every
 operation goes through the C ABI, and there is no CPU fallback.
 """
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -214,9 +215,10 @@ class DeviceBuffer:
         return self.t.dtype == torch.int64
 
 
-_RopeShape = C.c_uint64 * _lib.MAX_RANK
-_RopeStrides = C.c_int64 * _lib.MAX_RANK
-_OutStrides = C.c_int64 * 4
+@functools.lru_cache(maxsize=1024)
+def _rope_layout(shape, strides, out_strides):
+    """The ctypes arrays of a layout (read only): making them takes longer than the rest of a call."""
+    return ((C.c_uint64 * _lib.MAX_RANK)(*shape), (C.c_int64 * _lib.MAX_RANK)(*strides), (C.c_int64 * 4)(*out_strides))
 
 
 def _u64s(vals):
@@ -970,11 +972,12 @@ class CudaBackend:
             pp = self._want("rope: positions", positions, len(positions), i64=True)
             rows = 1 if len(positions) == s else b
         nx, no = len(x.buf), len(out.buf)
-        v = _lib.ViewDesc(self._want("rope: x", x.buf, nx), nx, x.offset, 4, _RopeShape(b, s, h, d), _RopeStrides(*x.strides))
+        c_shape, c_strides, c_out = _rope_layout(tuple(shape), tuple(x.strides), tuple(out.strides))
+        v = _lib.ViewDesc(self._want("rope: x", x.buf, nx), nx, x.offset, 4, c_shape, c_strides)
         self._call(self.lib.fb_rope, C.byref(v), pp, rows, start,
                                      self._want("rope: frequencies", plan.turns, plan.rot_dim // 2, i64=True), plan.rot_dim,
                                      plan.layout, plan.scale, inverse, self._want("rope: out", out.buf, no), no,
-                                     _OutStrides(*out.strides), out.offset)
+                                     c_out, out.offset)
         return out.buf
 
     def rope_dev(self, x, shape, plan: RopePlan, positions: Optional[DeviceBuffer] = None, start=0, out=None) -> DeviceBuffer:

@@ -609,60 +609,81 @@ moe_place_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
 // ---------------------------------------------------------------- rows
 constexpr int kRowThreads = 256;
 
-template <int VEC>
-struct RowVec {
+// What a thread moves of one row at a time: N accesses of VEC floats, `step` floats apart.  N is more
+// than 1 where rows fit no 16-byte access or a token has few choices, so that the bytes in flight stay.
+template <int VEC, int N>
+struct RowPart {
   static_assert(VEC == 1 || VEC == 2 || VEC == 4, "floats of one access");
-  float v[VEC];
-  __device__ __forceinline__ void load(const float* p) {
-    if constexpr (VEC == 4) {
-      const float4 t = ld_stream4(p);
-      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-    } else if constexpr (VEC == 2) {
-      const float2 t = __ldcs(reinterpret_cast<const float2*>(p));
-      v[0] = t.x; v[1] = t.y;
-    } else {
-      v[0] = ld_stream(p);
-    }
+  float v[N][VEC];
+  // The first access stands at p, the i-th exists where i < have.
+  __device__ __forceinline__ void load(const float* p, uint64_t step, uint32_t have) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < (int)have) {
+        const float* q = p + i * step;
+        if constexpr (VEC == 4) {
+          const float4 t = ld_stream4(q);
+          v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
+        } else if constexpr (VEC == 2) {
+          const float2 t = __ldcs(reinterpret_cast<const float2*>(q));
+          v[i][0] = t.x; v[i][1] = t.y;
+        } else {
+          v[i][0] = ld_stream(q);
+        }
+      }
   }
-  __device__ __forceinline__ void store(float* p) const {
-    if constexpr (VEC == 4) st_stream4(p, make_float4(v[0], v[1], v[2], v[3]));
-    else if constexpr (VEC == 2) __stcs(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
-    else st_stream(p, v[0]);
+  __device__ __forceinline__ void store(float* p, uint64_t step, uint32_t have) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < (int)have) {
+        float* q = p + i * step;
+        if constexpr (VEC == 4) st_stream4(q, make_float4(v[i][0], v[i][1], v[i][2], v[i][3]));
+        else if constexpr (VEC == 2) __stcs(reinterpret_cast<float2*>(q), make_float2(v[i][0], v[i][1]));
+        else st_stream(q, v[i][0]);
+      }
   }
 };
 
-// Where a thread stands.  A token's row is cut into vectors.  Narrow rows: a CTA takes `tpb` tokens, a
-// thread one vector.  Wider ones: a CTA takes a token, a thread every blockDim.x-th vector; where that
-// gives too few CTAs, one of `bpt` pieces of a token.  With 8192 tokens, 8 choices and 2048 columns the
-// gather runs at 102 % of the copy rate with a CTA per token and at 80 % with two CTAs per token, whose
-// halves of a row reach DRAM at different times.
+// Where a thread stands.  A row is cut into vectors of VEC floats; `width` threads share a token, thread l
+// of them takes vectors l, l + width, ... of its piece, N at a time.  Narrow rows: a CTA takes `tpb` tokens.
+// Wider ones: a CTA takes a token, or, where that gives too few CTAs, one of `bpt` pieces of a token.  With
+// 8192 tokens, 8 choices and 2048 columns the gather runs at 102 % of the copy rate with a CTA per token and
+// at 80 % with two CTAs per token, whose halves of a row reach DRAM at different times.
 struct RowMap {
   uint64_t tokens, cols, slots, blocks;
   uint32_t k, vpt;    // vectors per row
+  uint32_t width;     // threads per token
   uint32_t tpb, bpt;
   uint32_t piece;     // vectors per piece (bpt > 1)
-  FastDiv d_vpt;
+  FastDiv d_width;
 };
-// First vector of this thread, one behind its last, and their step; false: nothing to do.
+// Token and first vector of this thread and one behind the last of its piece; false: nothing to do.
 __device__ __forceinline__ bool row_place(const RowMap& M, uint64_t blk, uint64_t& t, uint32_t& vec, uint32_t& end) {
+  end = M.vpt;
   if (M.tpb > 1) {
-    const uint32_t tl = fdiv(threadIdx.x, M.d_vpt);
-    vec = threadIdx.x - tl * M.vpt;
-    end = vec + 1;
+    const uint32_t tl = fdiv(threadIdx.x, M.d_width);
+    vec = threadIdx.x - tl * M.width;
     t = blk * M.tpb + tl;
     return tl < M.tpb && t < M.tokens;
   }
-  if (M.bpt == 1) {
-    t = blk;
-    vec = threadIdx.x;
-    end = M.vpt;
-  } else {
+  vec = threadIdx.x;
+  t = blk;
+  if (M.bpt > 1) {
     t = blk / M.bpt;
     const uint32_t lo = (uint32_t)(blk - t * M.bpt) * M.piece;
-    vec = lo + threadIdx.x;
+    vec += lo;
     end = min(lo + M.piece, M.vpt);
   }
   return true;
+}
+// How many of a thread's next N vectors lie before `end`.
+template <int N>
+__device__ __forceinline__ uint32_t row_have(uint32_t vec, uint32_t end, uint32_t width) {
+  if (N == 1) return 1;
+  uint32_t have = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) have += vec + i * width < end;
+  return have;
 }
 
 __device__ __forceinline__ int64_t slot_of(const int64_t* place, uint64_t a, uint64_t slots) {
@@ -671,27 +692,29 @@ __device__ __forceinline__ int64_t slot_of(const int64_t* place, uint64_t a, uin
 }
 
 // xs[place[t, j]] = x[t], KU choices at a time: their places are loaded before the first store.
-template <int VEC, int KU>
-__global__ void __launch_bounds__(kRowThreads, KU == 8 ? 4 : 5)
+template <int VEC, int N, int KU>
+__global__ void __launch_bounds__(kRowThreads, KU == 8 ? 4 : KU == 4 ? 5 : 6)
 moe_scatter_kernel(const float* __restrict__ x, const int64_t* __restrict__ place, const __grid_constant__ RowMap M,
                    float* __restrict__ xs) {
   pdl_wait();
   pdl_trigger();
+  const uint64_t step = (uint64_t)M.width * VEC;
   for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
     uint64_t t;
     uint32_t vec, end;
     if (!row_place(M, blk, t, vec, end)) continue;
-    for (; vec < end; vec += blockDim.x) {
+    for (; vec < end; vec += M.width * N) {
       const uint64_t c = (uint64_t)vec * VEC;
-      RowVec<VEC> v;
-      v.load(x + t * M.cols + c);
+      const uint32_t have = row_have<N>(vec, end, M.width);
+      RowPart<VEC, N> v;
+      v.load(x + t * M.cols + c, step, have);
       for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
         int64_t s[KU];
 #pragma unroll
         for (int j = 0; j < KU; ++j) s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
 #pragma unroll
         for (int j = 0; j < KU; ++j)
-          if (s[j] >= 0) v.store(xs + (uint64_t)s[j] * M.cols + c);
+          if (s[j] >= 0) v.store(xs + (uint64_t)s[j] * M.cols + c, step, have);
       }
     }
   }
@@ -699,21 +722,25 @@ moe_scatter_kernel(const float* __restrict__ x, const int64_t* __restrict__ plac
 
 // y[t] = sum over j of (weights[t, j] *) ys[place[t, j]], KU rows in flight, added in the order of j.
 // Bound by HBM; what counts is enough CTAs per SM (five with KU 4) to cover the load of the places.
-template <int VEC, int KU, bool WEIGHTED>
-__global__ void __launch_bounds__(kRowThreads, KU == 8 ? 3 : 5)
+template <int VEC, int N, int KU, bool WEIGHTED>
+__global__ void __launch_bounds__(kRowThreads, KU == 8 ? 3 : N == 1 ? 5 : 4)
 moe_gather_kernel(const float* __restrict__ ys, const float* __restrict__ weights, const int64_t* __restrict__ place,
                   const __grid_constant__ RowMap M, float* __restrict__ y) {
   pdl_wait();
   pdl_trigger();
+  const uint64_t step = (uint64_t)M.width * VEC;
   for (uint64_t blk = blockIdx.x; blk < M.blocks; blk += gridDim.x) {
     uint64_t t;
     uint32_t vec, end;
     if (!row_place(M, blk, t, vec, end)) continue;
-    for (; vec < end; vec += blockDim.x) {
+    for (; vec < end; vec += M.width * N) {
       const uint64_t c = (uint64_t)vec * VEC;
-      RowVec<VEC> acc;
+      const uint32_t have = row_have<N>(vec, end, M.width);
+      RowPart<VEC, N> acc;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc.v[i] = 0.0f;
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc.v[n][i] = 0.0f;
       for (uint32_t j0 = 0; j0 < M.k; j0 += KU) {
         int64_t s[KU];
         float w[KU];
@@ -722,79 +749,105 @@ moe_gather_kernel(const float* __restrict__ ys, const float* __restrict__ weight
           s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
           if (WEIGHTED) w[j] = j0 + j < M.k ? __ldg(weights + t * M.k + j0 + j) : 0.0f;
         }
-        RowVec<VEC> r[KU];
+        RowPart<VEC, N> r[KU];
 #pragma unroll
         for (int j = 0; j < KU; ++j)
-          if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * M.cols + c);
+          if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * M.cols + c, step, have);
 #pragma unroll
         for (int j = 0; j < KU; ++j)
           if (s[j] >= 0) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc.v[i] = WEIGHTED ? fmaf(r[j].v[i], w[j], acc.v[i]) : acc.v[i] + r[j].v[i];
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+              for (int i = 0; i < VEC; ++i)
+                acc.v[n][i] = WEIGHTED ? fmaf(r[j].v[n][i], w[j], acc.v[n][i]) : acc.v[n][i] + r[j].v[n][i];
           }
       }
-      acc.store(y + t * M.cols + c);
+      acc.store(y + t * M.cols + c, step, have);
     }
   }
 }
 
 // dys[place[t, j]] = weights[t, j] * dy[t]; dweights[t, j] = dy[t] . ys[place[t, j]].  A token is owned by
-// a warp (WARP) or by the CTA, which walks the columns with KU rows of ys in flight; dy is read once per KU choices.
-// dys may be ys: an element is read by the thread that writes it, before it does.
-template <int VEC, int KU, bool WARP>
+// `lanes` lanes of a warp (a power of two; 0: by the CTA), which walk the columns with KU rows of ys in
+// flight; dy is read once per KU choices.  dys may be ys: an element is read by the thread that writes it,
+// before it does.
+template <int VEC, int N, int KU>
 __global__ void __launch_bounds__(kRowThreads, KU == 8 ? 2 : 3)
 moe_combine_bwd_kernel(const float* __restrict__ dy, const float* ys, const float* __restrict__ weights,
                        const int64_t* __restrict__ place, uint64_t tokens, uint32_t k, uint64_t cols, uint64_t slots,
-                       float* dys, float* __restrict__ dweights) {
+                       uint32_t lanes, float* dys, float* __restrict__ dweights) {
   pdl_wait();
   pdl_trigger();
   __shared__ float part[kRowThreads / 32][KU];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const uint64_t first = WARP ? (uint64_t)blockIdx.x * warps + warp : blockIdx.x;
-  const uint64_t step = WARP ? (uint64_t)gridDim.x * warps : gridDim.x;
-  const uint32_t l = WARP ? lane : threadIdx.x, width = WARP ? 32 : blockDim.x;
-  for (uint64_t t = first; t < tokens; t += step)
+  const uint32_t width = lanes ? lanes : blockDim.x, l = lanes ? lane & (lanes - 1) : threadIdx.x;
+  const uint32_t per_cta = lanes ? blockDim.x / lanes : 1, mine = lanes ? threadIdx.x / lanes : 0;
+  const uint32_t vpt = (uint32_t)(cols / VEC);
+  const uint64_t step = (uint64_t)width * VEC;
+  for (uint64_t t0 = (uint64_t)blockIdx.x * per_cta; t0 < tokens; t0 += (uint64_t)gridDim.x * per_cta) {
+    const uint64_t t = t0 + mine;
+    const bool live = t < tokens;  // all lanes meet in the sums below
     for (uint32_t j0 = 0; j0 < k; j0 += KU) {
       int64_t s[KU];
       float w[KU], dot[KU];
 #pragma unroll
       for (int j = 0; j < KU; ++j) {
-        s[j] = j0 + j < k ? slot_of(place, t * k + j0 + j, slots) : -1;
-        w[j] = j0 + j < k ? __ldg(weights + t * k + j0 + j) : 0.0f;
+        s[j] = live && j0 + j < k ? slot_of(place, t * k + j0 + j, slots) : -1;
+        w[j] = live && j0 + j < k ? __ldg(weights + t * k + j0 + j) : 0.0f;
         dot[j] = 0.0f;
       }
-      for (uint64_t c = (uint64_t)l * VEC; c < cols; c += (uint64_t)width * VEC) {
-        RowVec<VEC> g, r[KU];
-        g.load(dy + t * cols + c);
-        if (dweights) {
+      if (live) {
+        for (uint32_t vec = l; vec < vpt; vec += width * N) {
+          const uint64_t c = (uint64_t)vec * VEC;
+          const uint32_t have = row_have<N>(vec, vpt, width);
+          RowPart<VEC, N> g, r[KU];
+          g.load(dy + t * cols + c, step, have);
+          if (dweights) {
 #pragma unroll
-          for (int j = 0; j < KU; ++j)
-            if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * cols + c);
+            for (int j = 0; j < KU; ++j)
+              if (s[j] >= 0) r[j].load(ys + (uint64_t)s[j] * cols + c, step, have);
 #pragma unroll
-          for (int j = 0; j < KU; ++j)
-            if (s[j] >= 0) {
+            for (int j = 0; j < KU; ++j)
+              if (s[j] >= 0) {
 #pragma unroll
-              for (int i = 0; i < VEC; ++i) dot[j] = fmaf(g.v[i], r[j].v[i], dot[j]);
-            }
-        }
-        if (dys) {
+                for (int n = 0; n < N; ++n)
+                  if (n < (int)have) {
 #pragma unroll
-          for (int j = 0; j < KU; ++j)
-            if (s[j] >= 0) {
-              RowVec<VEC> o;
+                    for (int i = 0; i < VEC; ++i) dot[j] = fmaf(g.v[n][i], r[j].v[n][i], dot[j]);
+                  }
+              }
+          }
+          if (dys) {
 #pragma unroll
-              for (int i = 0; i < VEC; ++i) o.v[i] = g.v[i] * w[j];
-              o.store(dys + (uint64_t)s[j] * cols + c);
-            }
+            for (int j = 0; j < KU; ++j)
+              if (s[j] >= 0) {
+                RowPart<VEC, N> o;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                  for (int i = 0; i < VEC; ++i) o.v[n][i] = g.v[n][i] * w[j];
+                o.store(dys + (uint64_t)s[j] * cols + c, step, have);
+              }
+          }
         }
       }
       if (!dweights) continue;
+      if (lanes && lanes < 32) {
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+          for (uint32_t o = lanes / 2; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+          if (live && l == (uint32_t)j % lanes && j0 + j < k) dweights[t * k + j0 + j] = dot[j];
+        continue;
+      }
       const float sum = lanes_transpose_sum<32, KU>(dot, lane);  // choice lane / (32 / KU)
-      const uint32_t mine = lane / (32 / KU);
-      if (WARP) {
-        if (lane % (32 / KU) == 0 && j0 + mine < k) dweights[t * k + j0 + mine] = sum;
+      const uint32_t which = lane / (32 / KU);
+      if (lanes) {
+        if (live && lane % (32 / KU) == 0 && j0 + which < k) dweights[t * k + j0 + which] = sum;
       } else {
-        if (lane % (32 / KU) == 0) part[warp][mine] = sum;
+        if (lane % (32 / KU) == 0) part[warp][which] = sum;
         __syncthreads();
         if (threadIdx.x < KU && j0 + threadIdx.x < k) {
           float all = 0.0f;
@@ -804,6 +857,7 @@ moe_combine_bwd_kernel(const float* __restrict__ dy, const float* ys, const floa
         __syncthreads();
       }
     }
+  }
 }
 
 static int gate_check(const char* name, uint64_t tokens, uint64_t experts, uint64_t k) {
@@ -830,27 +884,31 @@ static int rows_check(const char* name, uint64_t tokens, uint64_t k, uint64_t co
 // token taken at once, for the shortest chain of loads instead of the best stream.
 static bool few_tokens(uint64_t tokens) { return tokens < (uint64_t)device_info().sm_count * 4; }
 
-static RowMap row_map(uint64_t tokens, uint64_t k, uint64_t cols, uint64_t slots, int vec, uint32_t* threads) {
+static RowMap row_map(uint64_t tokens, uint64_t k, uint64_t cols, uint64_t slots, int vec, int n, uint32_t* threads) {
   RowMap m = {};
   m.tokens = tokens;
   m.cols = cols;
   m.slots = slots;
   m.k = (uint32_t)k;
   m.vpt = (uint32_t)(cols / vec);
-  m.tpb = m.vpt <= kRowThreads / 2 ? kRowThreads / m.vpt : 1;
   m.bpt = 1;
-  m.d_vpt = make_fastdiv(m.vpt);
-  *threads = kRowThreads;
-  if (m.tpb == 1) {
-    // equal shares: as many threads as divide the row into the least number of rounds
-    const uint32_t rounds = (m.vpt + kRowThreads - 1) / kRowThreads;
-    *threads = ((m.vpt + rounds - 1) / rounds + 31) / 32 * 32;
+  const uint32_t most = kRowThreads * n, rounds = (m.vpt + most - 1) / most;
+  const uint32_t need = (m.vpt + rounds * n - 1) / (rounds * n);  // threads that divide a row into equal shares
+  if (need <= kRowThreads / 2) {
+    m.tpb = kRowThreads / need;
+    m.width = need;
+    *threads = kRowThreads;
+    m.blocks = (tokens + m.tpb - 1) / m.tpb;
+  } else {
+    m.tpb = 1;
+    m.width = *threads = (need + 31) / 32 * 32;
     if (rounds > 1 && few_tokens(tokens)) {
-      m.piece = *threads;
+      m.piece = m.width * n;
       m.bpt = (m.vpt + m.piece - 1) / m.piece;
     }
+    m.blocks = tokens * m.bpt;
   }
-  m.blocks = m.tpb > 1 ? (tokens + m.tpb - 1) / m.tpb : tokens * m.bpt;
+  m.d_width = make_fastdiv(m.width);
   return m;
 }
 
@@ -860,16 +918,18 @@ static int row_vec(uint64_t cols, const void* a, const void* b, const void* c = 
   return cols % 4 == 0 && at % 16 == 0 ? 4 : cols % 2 == 0 && at % 8 == 0 ? 2 : 1;
 }
 
+// Accesses per thread and row: 8 floats of each of two rows, 4 of more.
+static constexpr int row_n(int vec, int ku) { return (ku == 2 ? 8 : 4) / vec; }
 // CALL(VEC, KU) for the access width and the number of choices taken at a time.
-#define FB_ROW_KU(VEC, k, wide, CALL)  \
-  if ((k) <= 2) { CALL(VEC, 2); }      \
-  else if ((k) <= 4 || !(wide)) { CALL(VEC, 4); } \
+#define FB_ROW_KU(VEC, ku, CALL)         \
+  if ((ku) == 2) { CALL(VEC, 2); }       \
+  else if ((ku) == 4) { CALL(VEC, 4); }  \
   else { CALL(VEC, 8); }
-#define FB_ROW_DISPATCH(vec, k, wide, CALL)               \
-  do {                                                    \
-    if ((vec) == 4) { FB_ROW_KU(4, k, wide, CALL) }       \
-    else if ((vec) == 2) { FB_ROW_KU(2, k, wide, CALL) }  \
-    else { FB_ROW_KU(1, k, wide, CALL) }                  \
+#define FB_ROW_DISPATCH(vec, ku, CALL)             \
+  do {                                             \
+    if ((vec) == 4) { FB_ROW_KU(4, ku, CALL) }     \
+    else if ((vec) == 2) { FB_ROW_KU(2, ku, CALL) }\
+    else { FB_ROW_KU(1, ku, CALL) }                \
   } while (0)
 
 // CALL(L, V): lanes per token and values per lane that hold the experts of a row.
@@ -1024,12 +1084,12 @@ int fb_moe_dispatch_fwd(fb_stream_t stream, const float* x, const int64_t* place
   if (!x || !place || !xs) return fail(FB_ERR_INVALID_ARG, "%s: null buffer", name);
   if (overlaps(xs, slots * cols, x, tokens * cols) || overlaps(xs, slots * cols, place, 2 * tokens * k))
     return fail(FB_ERR_INVALID_ARG, "%s: xs must not overlap an input", name);
-  const int vec = row_vec(cols, x, xs);
+  const int vec = row_vec(cols, x, xs), ku = k <= 2 ? 2 : k <= 4 ? 4 : 8;
   uint32_t threads;
-  const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
+  const RowMap m = row_map(tokens, k, cols, slots, vec, row_n(vec, ku), &threads);
   const unsigned grid = grid_full(m.blocks);
-#define FB_CALL(VEC, KU) FB_CUDA(launch_pdl(moe_scatter_kernel<VEC, KU>, dim3(grid), dim3(threads), 0, stream, x, place, m, xs))
-  FB_ROW_DISPATCH(vec, k, true, FB_CALL);
+#define FB_CALL(VEC, KU) FB_CUDA(launch_pdl(moe_scatter_kernel<VEC, row_n(VEC, KU), KU>, dim3(grid), dim3(threads), 0, stream, x, place, m, xs))
+  FB_ROW_DISPATCH(vec, ku, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
@@ -1043,14 +1103,14 @@ static int gather_rows(cudaStream_t stream, const char* name, const float* ys, c
   if (overlaps(y, tokens * cols, ys, slots * cols) || overlaps(y, tokens * cols, weights, tokens * k) ||
       overlaps(y, tokens * cols, place, 2 * tokens * k))
     return fail(FB_ERR_INVALID_ARG, "%s: the output must not overlap an input", name);
-  const int vec = row_vec(cols, ys, y);
+  const int vec = row_vec(cols, ys, y), ku = k <= 2 ? 2 : k <= 4 || !few_tokens(tokens) ? 4 : 8;
   uint32_t threads;
-  const RowMap m = row_map(tokens, k, cols, slots, vec, &threads);
+  const RowMap m = row_map(tokens, k, cols, slots, vec, row_n(vec, ku), &threads);
   const unsigned grid = grid_full(m.blocks);
-#define FB_CALL(VEC, KU)                                                                                            \
-  if (weights) FB_CUDA(launch_pdl(moe_gather_kernel<VEC, KU, true>, dim3(grid), dim3(threads), 0, stream, ys, weights, place, m, y));            \
-  else FB_CUDA(launch_pdl(moe_gather_kernel<VEC, KU, false>, dim3(grid), dim3(threads), 0, stream, ys, weights, place, m, y))
-  FB_ROW_DISPATCH(vec, k, few_tokens(tokens), FB_CALL);
+#define FB_CALL(VEC, KU)                                                                                                   \
+  if (weights) FB_CUDA(launch_pdl(moe_gather_kernel<VEC, row_n(VEC, KU), KU, true>, dim3(grid), dim3(threads), 0, stream, ys, weights, place, m, y)); \
+  else FB_CUDA(launch_pdl(moe_gather_kernel<VEC, row_n(VEC, KU), KU, false>, dim3(grid), dim3(threads), 0, stream, ys, weights, place, m, y))
+  FB_ROW_DISPATCH(vec, ku, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
@@ -1080,16 +1140,25 @@ int fb_moe_combine_bwd(fb_stream_t stream, const float* dy, const float* ys, con
       overlaps(dweights, m, ys, n) || overlaps(dweights, m, dys, n) || overlaps(dweights, m, place, 2 * m))
     return fail(FB_ERR_INVALID_ARG, "%s: an output must not overlap another buffer, but dys may be ys", name);
   const int vec = row_vec(cols, dy, dweights ? ys : dy, dys);
-  // A warp per token up to 64 vectors a row, else a CTA with a thread per vector, at most 256.
-  const uint64_t vpt = cols / vec;
-  const bool by_warp = vpt <= 64;
-  const uint32_t threads = by_warp || vpt >= kRowThreads ? kRowThreads : (uint32_t)(vpt + 31) / 32 * 32;
-  const unsigned grid = grid_full(by_warp ? (tokens + kRowThreads / 32 - 1) / (kRowThreads / 32) : tokens);
+  const int ku = k <= 2 ? 2 : k <= 4 ? 4 : 8;
+  // Up to 64 threads' worth of a row: by a warp or as many of its lanes as have something to do.  Wider: by
+  // a CTA that divides the row into equal shares.
+  const uint32_t each = (uint32_t)row_n(vec, ku), vpt = (uint32_t)(cols / vec), most = kRowThreads * each;
+  const uint32_t need = (vpt + each - 1) / each, rounds = (vpt + most - 1) / most;
+  uint32_t lanes = 0, threads = kRowThreads;
+  if (need <= 64) {
+    for (lanes = 1; lanes < 32 && lanes < need; lanes <<= 1) {
+    }
+  } else {
+    threads = ((vpt + rounds * each - 1) / (rounds * each) + 31) / 32 * 32;
+  }
+  const uint32_t per_cta = lanes ? threads / lanes : 1;
+  const unsigned grid = grid_full((tokens + per_cta - 1) / per_cta);
   const uint32_t k32 = (uint32_t)k;
-#define FB_CALL(VEC, KU)                                                                                                              \
-  if (by_warp) FB_CUDA(launch_pdl(moe_combine_bwd_kernel<VEC, KU, true>, dim3(grid), dim3(threads), 0, stream, dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights)); \
-  else FB_CUDA(launch_pdl(moe_combine_bwd_kernel<VEC, KU, false>, dim3(grid), dim3(threads), 0, stream, dy, ys, weights, place, tokens, k32, cols, slots, dys, dweights))
-  FB_ROW_DISPATCH(vec, k, true, FB_CALL);
+#define FB_CALL(VEC, KU) \
+  FB_CUDA(launch_pdl(moe_combine_bwd_kernel<VEC, row_n(VEC, KU), KU>, dim3(grid), dim3(threads), 0, stream, dy, ys, weights, place, \
+                     tokens, k32, cols, slots, lanes, dys, dweights))
+  FB_ROW_DISPATCH(vec, ku, FB_CALL);
 #undef FB_CALL
   FB_LAUNCHED(name);
   return FB_OK;
