@@ -279,6 +279,50 @@ def cases(B, only, small=False, widths=None):
         B.run("c5_mse_fwd_bwd [65536,4096]", 3 * r * c * 4,
               lambda: be._check(lib.fb_mse_fwd_bwd(S(), p.ptr, t.ptr, r * c, 1.0, loss.ptr, dp.ptr, ws.ptr, len(ws) * 4)))
 
+    # ---- what a transformer layer with routed experts runs between its matrix products (not in the default table: run with --only layer)
+    if only is not None and want("layer"):
+        layer_cases(B, small)
+
+
+def layer_cases(B, small):
+    be = B.be
+    d = 8 if small else 1
+    for heads, dim, rot, layout in [(32, 128, 128, "interleaved"), (32, 128, 128, "half"), (32, 80, 40, "half"), (8, 256, 64, "half"), (25, 126, 126, "half"), (1, 128, 128, "half")]:
+        t = 16384 // d * (32 // heads if heads < 25 else 1)
+        shape, n = (1, t, heads, dim), t * heads * dim
+        x, out, plan = B.randn(n), B.empty(n), be.rope_plan(rot, layout=layout)
+        B.run(f"layer_rope [{t},{heads},{dim}] {rot} channels, {layout}", 8 * n, lambda: be.rope_dev(x, shape, plan, out=out))
+        del x, out
+    for rows, cols in [(16384 // d, 4096), (16384 // d, 4095), (1048576 // d, 64)]:
+        n = rows * cols
+        x, r, b, out, db = B.randn(n), B.randn(n), B.randn(cols), B.empty(n), B.empty(cols)
+        B.run(f"layer_dropout_fwd [{rows},{cols}]", 8 * n, lambda: be.dropout_dev(x, None, None, 0.1, 1, 2, rows, cols, out=out))
+        B.run(f"layer_dropout_fwd bias, residual [{rows},{cols}]", 12 * n, lambda: be.dropout_dev(x, b, r, 0.1, 1, 2, rows, cols, out=out))
+        B.run(f"layer_dropout_bwd dx,db [{rows},{cols}]", 8 * n, lambda: be.dropout_backward_dev(x, 0.1, 1, 2, rows, cols, dx=out, dbias=db))
+        del x, r, out
+    for t, e, k in [(32768, 128, 8), (32768, 64, 2), (32768, 256, 8), (32768, 128, 16)]:
+        t //= d
+        l, w, dw, dl, ids = B.randn(t * e), B.empty(t * k), B.randn(t * k), B.empty(t * e), B.empty(t * k, torch.int64)
+        for renorm in (True, False):
+            what = "chosen" if renorm else "all"
+            B.run(f"layer_gate_fwd softmax over {what} [{t},{e}] k {k}", 4 * t * e + 12 * t * k,
+                  lambda: be.moe_gate_dev(l, t, e, k, renorm, weights=w, ids=ids))
+            B.run(f"layer_gate_bwd softmax over {what} [{t},{e}] k {k}", (1 if renorm else 2) * 4 * t * e + 16 * t * k,
+                  lambda: be.moe_gate_backward_dev(dw, l, w, ids, t, e, k, renorm, dlogits=dl))
+    for t, e, k, c in [(8192, 128, 8, 2048), (32768, 64, 2, 1024), (16384, 64, 6, 1001)]:
+        t //= d
+        n = t * k
+        l, x, xs, ys, y, dw = B.randn(t * e), B.randn(t * c), B.empty(n * c), B.randn(n * c), B.empty(t * c), B.empty(n)
+        w, ids = be.moe_gate_dev(l, t, e, k)
+        plan = be.moe_sort_dev(ids, t, k, e)
+        rows = 4 * c * (n + t) + 8 * n
+        B.run(f"layer_expert_sort [{t},{k}] {e} experts", 24 * n, lambda: be.moe_sort_dev(ids, t, k, e, place=plan.place, order=plan.order, offsets=plan.offsets))
+        B.run(f"layer_dispatch_fwd [{t},{k},{c}]", rows, lambda: be.moe_dispatch_dev(x, plan, c, out=xs))
+        B.run(f"layer_dispatch_bwd [{t},{k},{c}]", rows, lambda: be.moe_dispatch_backward_dev(ys, plan, c, out=y))
+        B.run(f"layer_combine_fwd [{t},{k},{c}]", rows + 4 * n, lambda: be.moe_combine_dev(ys, w, plan, c, out=y))
+        B.run(f"layer_combine_bwd [{t},{k},{c}]", 4 * c * (2 * n + t) + 16 * n, lambda: be.moe_combine_backward_dev(x, ys, w, plan, c, dys=xs, dweights=dw))
+        del x, xs, ys, y
+
 
 def main():
     ap = argparse.ArgumentParser()

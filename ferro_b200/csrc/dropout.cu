@@ -296,32 +296,31 @@ dropout_bwd_kernel(const float* g, uint64_t n, uint32_t cols, const __grid_const
   }
 }
 
-// dbias[c] = sum over rows of part[row][c]: eight threads per column take every eighth row, then a fixed
-// order.
-__global__ void __launch_bounds__(256)
+// dbias[c] = sum over rows of part[row][c]: 32 threads per column take every 32nd row, then a fixed order.
+// A chain of loads whatever it does; eight threads per column took 8.3 us for 293 rows of 64, this 4 to 5.
+__global__ void __launch_bounds__(1024)
 dropout_bias_kernel(const float* __restrict__ part, uint32_t rows, uint64_t cols, float* __restrict__ dbias) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float sm[8][32];
+  __shared__ float sm[32][33];
   const uint32_t lane = threadIdx.x & 31, y = threadIdx.x >> 5;
   const uint64_t c = (uint64_t)blockIdx.x * 32 + lane;
   float t = 0.0f;
   if (c < cols) {
     uint32_t s = y;
-    for (; s + 24 < rows; s += 32) {
-      const float a = __ldcg(part + (uint64_t)s * cols + c), b = __ldcg(part + (uint64_t)(s + 8) * cols + c);
-      const float d = __ldcg(part + (uint64_t)(s + 16) * cols + c), f = __ldcg(part + (uint64_t)(s + 24) * cols + c);
+    for (; s + 96 < rows; s += 128) {
+      const float a = __ldcg(part + (uint64_t)s * cols + c), b = __ldcg(part + (uint64_t)(s + 32) * cols + c);
+      const float d = __ldcg(part + (uint64_t)(s + 64) * cols + c), f = __ldcg(part + (uint64_t)(s + 96) * cols + c);
       t = (((t + a) + b) + d) + f;
     }
-    for (; s < rows; s += 8) t += __ldcg(part + (uint64_t)s * cols + c);
+    for (; s < rows; s += 32) t += __ldcg(part + (uint64_t)s * cols + c);
   }
   sm[y][lane] = t;
   __syncthreads();
-  if (y == 0 && c < cols) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) t += sm[i][lane];
-    dbias[c] = t;
-  }
+  // warp y adds up column y of the CTA's 32
+  const float sum = warp_sum(sm[lane][y]);
+  const uint64_t mine = (uint64_t)blockIdx.x * 32 + y;
+  if (lane == 0 && mine < cols) dbias[mine] = sum;
 }
 
 __global__ void dropout_advance_kernel(int64_t* counter, uint64_t n) {
@@ -432,7 +431,7 @@ int fb_dropout_bwd(fb_stream_t stream, const float* g, uint64_t rows, uint64_t c
   else FB_CUDA(launch_pdl(dropout_bwd_kernel<false, false>, dim3(grid), dim3(kDropThreads), 0, stream, g, n, (uint32_t)cols, plan, m, dx, sums));
   FB_LAUNCHED(name);
   if (need) {
-    FB_CUDA(launch_pdl(dropout_bias_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(256), 0, stream, (const float*)sums,
+    FB_CUDA(launch_pdl(dropout_bias_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, stream, (const float*)sums,
                        (uint32_t)plan.sum_rows, cols, dbias));
     FB_LAUNCHED(name);
   }
