@@ -1090,7 +1090,8 @@ class CudaBackend:
         return len(buf) // cols
 
     def moe_dispatch_dev(self, x, plan: MoePlan, cols, out=None) -> DeviceBuffer:
-        """xs[place[t, j]] = x[t]; rows of xs behind the last assignment are left as they were."""
+        """xs[place[t, j]] = x[t]; rows of xs behind the last assignment are left as they were (in a buffer allocated here:
+        uninitialised)."""
         px = self._want("moe_dispatch: x", x, plan.tokens * cols)
         if out is None:
             out = self._alloc(plan.tokens * plan.k * cols)
@@ -1121,7 +1122,8 @@ class CudaBackend:
 
     def moe_combine_backward_dev(self, g, ys, weights, plan: MoePlan, cols, want_dys=True, want_dweights=True, dys=None,
                                  dweights=None):
-        """(dys | None, dweights | None); rows of dys behind the last assignment are left as they were; dys may be ys."""
+        """(dys | None, dweights | None); rows of dys behind the last assignment are left as they were (in a buffer allocated
+        here: uninitialised); dys may be ys."""
         pg, pw = self._want("moe_combine_backward: g", g, plan.tokens * cols), self._want("moe_combine_backward: weights", weights, plan.tokens * plan.k)
         rows = self._moe_rows("moe_combine_backward", ys, cols)
         if dys is None and want_dys:

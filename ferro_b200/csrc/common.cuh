@@ -100,7 +100,10 @@ inline unsigned grid_full(uint64_t work_items) {
 // this one has passed it (or exited), so it costs this kernel nothing.  A
 // kernel that never triggers releases its dependents when it ends, and a
 // predecessor that is not ours behaves exactly like that: ordering is never
-// weaker than plain stream order.
+// weaker than plain stream order.  A predecessor may still be writing operands
+// when the kernel becomes resident: rope.cu, dropout.cu and moe.cu read them with
+// coherent loads (ld.global, which pdl_wait() orders) and not through the
+// read-only path, whose data must not change during the kernel.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -25,7 +25,7 @@ struct DropMask {
   const int64_t* counter;
   uint32_t least;  // smallest word that keeps its element
   float factor;    // 1 / (1 - p)
-  __device__ __forceinline__ uint64_t first() const { return offset + (counter ? (uint64_t)__ldg(counter) : 0ull); }
+  __device__ __forceinline__ uint64_t first() const { return offset + (counter ? (uint64_t)__ldca(counter) : 0ull); }
   __device__ __forceinline__ bool keep(uint32_t word) const { return word >= least; }
 };
 
@@ -70,12 +70,12 @@ dropout_kernel(const float* x, const float* __restrict__ bias, const float* resi
       if (BIAS != DROP_NO_BIAS) {
         uint32_t c = (e >> 32) ? (uint32_t)(e % cols) : (uint32_t)e - fdiv((uint32_t)e, d_cols) * cols;
         if (BIAS == DROP_BIAS_VEC) {
-          const float4 b = __ldg(reinterpret_cast<const float4*>(bias + c));
+          const float4 b = __ldca(reinterpret_cast<const float4*>(bias + c));
           v[k][0] += b.x; v[k][1] += b.y; v[k][2] += b.z; v[k][3] += b.w;
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            v[k][j] += __ldg(bias + c);
+            v[k][j] += __ldca(bias + c);
             if (++c == cols) c = 0;
           }
         }

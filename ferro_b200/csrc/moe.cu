@@ -13,10 +13,10 @@
 namespace fb {
 
 // ---------------------------------------------------------------- gate
-// One warp per token; lane l holds experts l, l + 32, ...  A logit is turned into
-// an unsigned key whose order is the order of choice: -inf (masked) lowest, then
-// the finite values ascending, +inf, NaN highest.  Adding +0 first makes -0 and
-// +0 the same key and every NaN the one positive NaN the adder returns.
+// A logit is turned into an unsigned key whose order is the order of choice: -inf
+// (masked) lowest, then the finite values ascending, +inf, NaN highest.  Adding +0
+// first makes -0 and +0 the same key and every NaN the one positive NaN the adder
+// returns.
 constexpr uint32_t kGateMasked = 0x007fffffu;  // the key of -inf
 __device__ __forceinline__ uint32_t gate_key(float v) {
   const int32_t u = __float_as_int(v + 0.0f);
@@ -37,7 +37,7 @@ __device__ __forceinline__ int32_t gate_choose_exact(const float* __restrict__ r
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
     const uint32_t e = i * 32 + lane;
-    key[i] = e < experts ? gate_key(__ldg(row + e)) : 0u;
+    key[i] = e < experts ? gate_key(__ldca(row + e)) : 0u;
   }
   int32_t mine = -1;
   for (uint32_t j = 0; j < k; ++j) {
@@ -138,7 +138,7 @@ __device__ __forceinline__ void gate_load(const float* __restrict__ row, uint32_
 #pragma unroll
     for (int r = 0; r < V; r += 4) {
       const uint32_t e = gate_expert<L, V>(r, l, true);
-      const float4 t = live && e < experts ? __ldg(reinterpret_cast<const float4*>(row + e)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      const float4 t = live && e < experts ? __ldca(reinterpret_cast<const float4*>(row + e)) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       v[r] = t.x;
       if constexpr (V % 4 == 0) { v[r + 1] = t.y; v[r + 2] = t.z; v[r + 3] = t.w; }
     }
@@ -146,7 +146,7 @@ __device__ __forceinline__ void gate_load(const float* __restrict__ row, uint32_
 #pragma unroll
     for (int r = 0; r < V; ++r) {
       const uint32_t e = r * L + l;
-      v[r] = live && e < experts ? __ldg(row + e) : -INFINITY;
+      v[r] = live && e < experts ? __ldca(row + e) : -INFINITY;
     }
   }
 }
@@ -167,7 +167,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // kept bits with the last chosen.  Such a token is chosen again on whole keys by the whole warp.
 //
 // Bound by the integer pipe, which issues half the rate of the others: per token of 128 experts and 8
-// choices about 100 instructions, 12 us for 32768 tokens; one warp-wide maximum per choice took 407 (16 us).
+// choices 190 instructions, 11.6 us for 32768 tokens; one warp-wide maximum per choice took 407 (16 us).
 template <int KL, int L, int V>
 __global__ void __launch_bounds__(kGateThreads, V <= 16 ? 8 : 4)
 moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t experts, uint32_t k, bool renorm, bool vec,
@@ -211,7 +211,7 @@ moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t 
     }
     const bool mine_in = l < (int)k && mine > kGateMasked;
     int32_t id = mine_in ? (int32_t)(kIds - 1 - (mine & (kIds - 1))) : -1;
-    float value = mine_in ? __ldg(row + id) : 0.0f;
+    float value = mine_in ? __ldca(row + id) : 0.0f;
     const float after_value = __shfl_down_sync(0xffffffffu, value, 1);
     bool clash = false;
     if (mine_in && l + 1 < (int)k && after > kGateMasked)
@@ -233,7 +233,7 @@ moe_gate_fwd_kernel(const float* __restrict__ logits, uint64_t tokens, uint32_t 
       const int32_t theirs = __shfl_sync(0xffffffffu, found, l);
       if (g == who) {
         id = l < (int)k ? theirs : -1;
-        value = id >= 0 ? __ldg(row + id) : 0.0f;
+        value = id >= 0 ? __ldca(row + id) : 0.0f;
       }
     }
     const float m = __shfl_sync(0xffffffffu, value, g * L);  // the largest, where there is one
@@ -298,7 +298,7 @@ moe_gate_fwd_many_kernel(const float* __restrict__ logits, uint64_t tokens, uint
     }
     const bool in = mine > kGateMasked;  // lanes from k on hold 0
     int32_t id = in ? (int32_t)(kIds - 1 - (mine & (kIds - 1))) : -1;
-    float value = in ? __ldg(row + id) : 0.0f;
+    float value = in ? __ldca(row + id) : 0.0f;
     uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
     const float after_value = __shfl_down_sync(0xffffffffu, value, 1);
     bool clash = in && (uint32_t)lane + 1 < k && after > kGateMasked && ((mine ^ after) & kKept) == 0 &&
@@ -306,7 +306,7 @@ moe_gate_fwd_many_kernel(const float* __restrict__ logits, uint64_t tokens, uint
     clash |= in && (uint32_t)lane + 1 == k && next > kGateMasked && ((mine ^ next) & kKept) == 0;
     if (__any_sync(0xffffffffu, clash)) {
       id = gate_choose_exact<NPL>(row, experts, k, lane);
-      value = id >= 0 ? __ldg(row + id) : 0.0f;
+      value = id >= 0 ? __ldca(row + id) : 0.0f;
     }
     const float m = __shfl_sync(0xffffffffu, value, 0);
     const float mass = id >= 0 ? gate_exp(value - m) : 0.0f;
@@ -352,11 +352,11 @@ moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict_
       id[i] = -1;
       w[i] = dw[i] = 0.0f;
       if (live && j < k) {
-        const int64_t e = __ldg(ids + t * k + j);
+        const int64_t e = __ldca(ids + t * k + j);
         if (e >= 0 && e < (int64_t)experts) {
           id[i] = (int32_t)e;
-          w[i] = __ldg(weights + t * k + j);
-          dw[i] = __ldg(dweights + t * k + j);
+          w[i] = __ldca(weights + t * k + j);
+          dw[i] = __ldca(dweights + t * k + j);
           dot = fmaf(w[i], dw[i], dot);
         }
       }
@@ -419,7 +419,7 @@ moe_gate_bwd_kernel(const float* __restrict__ dweights, const float* __restrict_
 // ---------------------------------------------------------------- sort
 // Counting sort.  A CTA owns a chunk of neighbouring assignments, a warp 32 * R of them.  Within a
 // warp the rank of an assignment among those of its expert comes from the lanes that hold the same id
-// (match) plus the warp's running count; between warps and chunks counts are summed in order.
+// (ballots) plus the warp's running count; between warps and chunks counts are summed in order.
 constexpr int kSortThreads = 1024;
 constexpr int kSortRounds = 4;  // R where one assignment per thread would take too many chunks
 
@@ -451,7 +451,7 @@ moe_count_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint32_t i = base + r * kSortThreads + threadIdx.x;
-    id[r] = i < n ? sort_id(__ldg(ids + i), experts) : experts;
+    id[r] = i < n ? sort_id(__ldca(ids + i), experts) : experts;
   }
   for (uint32_t e = threadIdx.x; e < experts; e += kSortThreads) hist[e] = 0;
   __syncthreads();
@@ -517,7 +517,7 @@ moe_place_kernel(const int64_t* __restrict__ ids, uint32_t n, uint32_t experts, 
     const uint32_t i = base + r * 32;
     id[r] = experts;
     if (i < n) {
-      const int64_t e = __ldg(ids + i);
+      const int64_t e = __ldca(ids + i);
       id[r] = sort_id(e, experts);
       if (id[r] == experts && e != -1 && bad) atomicMax(reinterpret_cast<long long*>(bad), (long long)i + 1);
     }
@@ -687,7 +687,7 @@ __device__ __forceinline__ uint32_t row_have(uint32_t vec, uint32_t end, uint32_
 }
 
 __device__ __forceinline__ int64_t slot_of(const int64_t* place, uint64_t a, uint64_t slots) {
-  const int64_t s = __ldg(place + a);
+  const int64_t s = __ldca(place + a);
   return s >= 0 && (uint64_t)s < slots ? s : -1;
 }
 
@@ -747,7 +747,7 @@ moe_gather_kernel(const float* __restrict__ ys, const float* __restrict__ weight
 #pragma unroll
         for (int j = 0; j < KU; ++j) {
           s[j] = j0 + j < M.k ? slot_of(place, t * M.k + j0 + j, M.slots) : -1;
-          if (WEIGHTED) w[j] = j0 + j < M.k ? __ldg(weights + t * M.k + j0 + j) : 0.0f;
+          if (WEIGHTED) w[j] = j0 + j < M.k ? __ldca(weights + t * M.k + j0 + j) : 0.0f;
         }
         RowPart<VEC, N> r[KU];
 #pragma unroll
@@ -794,7 +794,7 @@ moe_combine_bwd_kernel(const float* __restrict__ dy, const float* ys, const floa
 #pragma unroll
       for (int j = 0; j < KU; ++j) {
         s[j] = live && j0 + j < k ? slot_of(place, t * k + j0 + j, slots) : -1;
-        w[j] = live && j0 + j < k ? __ldg(weights + t * k + j0 + j) : 0.0f;
+        w[j] = live && j0 + j < k ? __ldca(weights + t * k + j0 + j) : 0.0f;
         dot[j] = 0.0f;
       }
       if (live) {

@@ -137,10 +137,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
         if (kTwo && second) rope_load<VEC>(xb + (int64_t)h * A.xs[2], vb[h]);
       }
     if (turn) {
-      const uint64_t p = A.pos ? (uint64_t)__ldg(A.pos + (A.pos_batch ? token : s)) : (uint64_t)A.start + s;
+      const uint64_t p = A.pos ? (uint64_t)__ldca(A.pos + (A.pos_batch ? token : s)) : (uint64_t)A.start + s;
       float sn[kPairs], cs[kPairs];
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) turn_sincos(p * (uint64_t)__ldg(A.turns + pair + i), A.scale, A.flip, sn[i], cs[i]);
+      for (int i = 0; i < kPairs; ++i) turn_sincos(p * (uint64_t)__ldca(A.turns + pair + i), A.scale, A.flip, sn[i], cs[i]);
 #pragma unroll
       for (int h = 0; h < HPT; ++h)
         if (h < (int)hn) {
