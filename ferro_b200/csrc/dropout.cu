@@ -111,9 +111,10 @@ dropout_kernel(const float* x, const float* __restrict__ bias, const float* resi
 // adds the rows in order.
 //
 // Bound by HBM as far as a grid of resident CTAs allows that reads and writes in equal measure: 16384 x
-// 4096 in 97 us, 84 % of the copy rate.  Seven groups are in flight per thread while seven go through the
+// 4096 in 95 us, 87 % of the copy rate.  Seven groups are in flight per thread while seven go through the
 // generator, on two CTAs per SM; four on three, four or five CTAs took 103 to 125 us, without the early
-// loads 109 us at best, a column sum that draws the mask at each load 107 us.
+// loads 109 us at best, a column sum that draws the mask at each load 107 us, staging through shared
+// memory by bulk copies (2 to 8 stages of 8 KB, 3 to 8 CTAs per SM) 94 to 113 us.
 constexpr int kDropBwdUnroll = 7;      // groups in flight per thread: 8 spill
 constexpr int kDropBwdPerSm = 2;       // CTAs, by registers
 constexpr uint32_t kDropTile = kDropThreads * 4;

@@ -205,6 +205,31 @@ def test_dropout_forward_and_gradient(be, rows, cols, bias, residual):
     assert (bits(be.copy_to_host(G).reshape(rows, cols)) == bits(gdx)).all()
 
 
+@pytest.mark.parametrize("rows,cols", [(15000, 1001), (3800, 4100), (16384, 1024), (20000, 1030), (500000, 33), (2500000, 7), (17000001, 1), (9000, 2049), (160, 100000)])
+def test_dropout_gradient_of_large_matrices(be, rows, cols):
+    """Sizes at which every thread has many groups: dx is what the forward kernel makes of g bit for bit, the bias gradient
+    is dx's column sum, with and without dx, in place, and from an address that fits no vector."""
+    DeviceBuffer = bk().DeviceBuffer
+    n, p, seed, off = rows * cols, 0.3, 2 ** 63 + 5, 2 ** 32 - 100
+    with torch.cuda.stream(be.stream):
+        gen = torch.Generator(device=be.device).manual_seed(cols)
+        hold = torch.randn(n + 4, device=be.device, generator=gen)
+        G, shifted = DeviceBuffer(hold[:n].clone()), DeviceBuffer(hold[1:n + 1])
+        shifted.t.copy_(G.t)
+    want = be.dropout_dev(G, None, None, p, seed, off, rows, cols)
+    dx, db = be.dropout_backward_dev(G, p, seed, off, rows, cols, want_dbias=True)
+    _, only = be.dropout_backward_dev(G, p, seed, off, rows, cols, want_dx=False, want_dbias=True)
+    sdx, sdb = be.dropout_backward_dev(shifted, p, seed, off, rows, cols, want_dbias=True)
+    be.dropout_backward_dev(G, p, seed, off, rows, cols, want_dbias=True, dx=G)
+    be.synchronize()
+    assert torch.equal(dx.t, want.t) and torch.equal(sdx.t, want.t) and torch.equal(G.t, want.t)
+    assert torch.equal(db.t, only.t)
+    m = want.t.view(rows, cols).double()
+    # a column's sum is at most 256 additions deep: blocks in a thread, threads of a CTA, rows of partial sums
+    bound = 256 * EPS * m.abs().sum(0)
+    assert bool(((db.t.double() - m.sum(0)).abs() <= bound).all()) and bool(((sdb.t.double() - m.sum(0)).abs() <= bound).all())
+
+
 @pytest.mark.parametrize("n,shift", [(1000, 1), (4097, 2), (64, 3), (5, 1)])
 def test_dropout_at_addresses_that_fit_no_vector(be, n, shift):
     """The mask goes by element number, not by address."""
