@@ -489,9 +489,9 @@ moe_scan_kernel(uint32_t* __restrict__ counts, uint32_t chunks, uint32_t experts
 }
 
 // How a CTA learns what the other chunks hold: there are none; it adds up the counts of all chunks
-// (kSortDirect at most); moe_scan_kernel has left prefixes and totals.
+// (kSortDirect chunks and kSortCounts counts at most); moe_scan_kernel has left prefixes and totals.
 enum { SORT_ALONE = 0, SORT_DIRECT = 1, SORT_SCANNED = 2 };
-constexpr uint32_t kSortDirect = 64;
+constexpr uint32_t kSortDirect = 128, kSortCounts = 32768;
 
 // blockDim.x is a multiple of 32 and at least `experts`.
 template <int R>
@@ -958,9 +958,11 @@ static constexpr int row_n(int vec, int ku) { return (ku == 2 ? 8 : 4) / vec; }
     else { CALL(32); }                             \
   } while (0)
 
-// One CTA up to 4096 assignments.  Beyond, chunks of 1024 (a thread each) while their counts can be added up
-// by every CTA, else of 4096: 65536 assignments to 128 experts take 6.1 us in 64 chunks (when the choice was
-// made 8.3, against 15.8 in 16).
+// One CTA up to 4096 assignments (one launch; two take less time on the GPU but more on the host).  Beyond,
+// chunks of 1024 (a thread each) up to kSortDirect of them, else of 4096; every CTA adds the counts up itself
+// while there are few.  131072 assignments to 64 / 128 / 256 experts take 6.8 / 7.1 / 9.5 us in 128 chunks,
+// 9.4 / 10.2 / 11.4 in 32; to 1024 experts 23.8 against 18.6.  With 128 chunks of 4096 and 1024 experts the
+// scan of its own takes 20.1 us, adding up in every CTA 27.7.
 struct SortPlan {
   uint32_t rounds, threads, chunks;
   int mode;
@@ -968,11 +970,11 @@ struct SortPlan {
 static SortPlan sort_plan(uint64_t n, uint64_t experts) {
   SortPlan p;
   const uint64_t most = n > experts ? n : experts;
-  p.rounds = n <= kSortThreads || (n > kSortThreads * kSortRounds && n <= (uint64_t)kSortThreads * kSortDirect) ? 1 : kSortRounds;
+  p.rounds = n <= kSortThreads || (n > kSortThreads * kSortRounds && n <= (uint64_t)kSortThreads * kSortDirect && experts <= 512) ? 1 : kSortRounds;
   p.threads = most < kSortThreads ? (uint32_t)(most + 31) / 32 * 32 : kSortThreads;
   const uint64_t chunk = (uint64_t)p.threads * p.rounds;
   p.chunks = n ? (uint32_t)((n + chunk - 1) / chunk) : 1;
-  p.mode = p.chunks == 1 ? SORT_ALONE : p.chunks <= kSortDirect ? SORT_DIRECT : SORT_SCANNED;
+  p.mode = p.chunks == 1 ? SORT_ALONE : p.chunks <= kSortDirect && p.chunks * experts <= kSortCounts ? SORT_DIRECT : SORT_SCANNED;
   return p;
 }
 
