@@ -11,6 +11,7 @@ operation goes through the C ABI, and there is no CPU fallback.
 """
 import ctypes as C
 import functools
+import threading
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -249,12 +250,21 @@ class CudaBackend:
         torch.cuda.set_device(self.device)
         # One non-default stream per backend, like lib.rs:308-312.
         self.stream = torch.cuda.Stream(device=self.device)
-        self._stream_handle = C.c_void_p(self.stream.cuda_stream)
         self._ws = None
+        self._scratch_lock = threading.Lock()  # see _call_with_scratch
         with torch.cuda.stream(self.stream):
             self._bad_expert = torch.zeros(1, dtype=torch.int64, device=self.device)  # see check_experts
 
     # -- plumbing ---------------------------------------------------------------
+    @property
+    def stream(self):
+        return self._stream
+
+    @stream.setter
+    def stream(self, stream):
+        self._stream, self._stream_handle = stream, C.c_void_p(stream.cuda_stream)
+        self._scratch = None  # the old stream's work may still be in it
+
     def _s(self):
         return self._stream_handle
 
@@ -921,16 +931,23 @@ class CudaBackend:
         if rc != 0:
             self._check(rc)
 
-    def _scratch(self, nbytes):
-        """(address, bytes, owner) of one call's scratch: the backend's own on its stream, but memory of the graph's pool
-        during a capture, so that graphs share none with each other or with eager calls."""
+    def _call_with_scratch(self, nbytes, fn, *args):
+        """_call with (scratch, bytes) behind the arguments.  The backend's own scratch is handed out under a lock: a call's
+        launches stand together on the stream, whatever other threads do.  During a capture it is memory of the graph's
+        pool, so that graphs share none with each other or with eager calls."""
         if not nbytes:
-            return None, 0, None
-        if torch.cuda.is_current_stream_capturing():
+            self._call(fn, *args, None, 0)
+        elif torch.cuda.is_current_stream_capturing():
             with torch.cuda.stream(self.stream):
                 t = torch.empty(int(nbytes), dtype=torch.uint8, device=self.device)
-            return t.data_ptr(), int(nbytes), t
-        return (*self._workspace(nbytes), None)
+            self._call(fn, *args, t.data_ptr(), int(nbytes))
+        else:
+            with self._scratch_lock:
+                t = self._scratch
+                if t is None or t.numel() < nbytes:
+                    with torch.cuda.stream(self.stream):
+                        t = self._scratch = torch.empty(max(int(nbytes), 1 << 20), dtype=torch.uint8, device=self.device)
+                self._call(fn, *args, t.data_ptr(), t.numel())
 
     # -- rotary positions ---------------------------------------------------------------------------------
     ROPE_LAYOUTS = {"interleaved": K.ROPE_INTERLEAVED, "half": K.ROPE_HALF}
@@ -975,9 +992,9 @@ class CudaBackend:
         c_shape, c_strides, c_out = _rope_layout(tuple(shape), tuple(x.strides), tuple(out.strides))
         v = _lib.ViewDesc(self._want("rope: x", x.buf, nx), nx, x.offset, 4, c_shape, c_strides)
         self._call(self.lib.fb_rope, C.byref(v), pp, rows, start,
-                                     self._want("rope: frequencies", plan.turns, plan.rot_dim // 2, i64=True), plan.rot_dim,
-                                     plan.layout, plan.scale, inverse, self._want("rope: out", out.buf, no), no,
-                                     c_out, out.offset)
+                   self._want("rope: frequencies", plan.turns, plan.rot_dim // 2, i64=True), plan.rot_dim,
+                   plan.layout, plan.scale, inverse, self._want("rope: out", out.buf, no), no,
+                   c_out, out.offset)
         return out.buf
 
     def rope_dev(self, x, shape, plan: RopePlan, positions: Optional[DeviceBuffer] = None, start=0, out=None) -> DeviceBuffer:
@@ -1007,7 +1024,7 @@ class CudaBackend:
         if out is None:
             out = self._alloc(n)
         self._call(self.lib.fb_dropout_fwd, px, pb, pr, rows, cols, p, seed, offset, pc,
-                                            self._want("dropout: out", out, n))
+                   self._want("dropout: out", out, n))
         return out
 
     def dropout_backward_dev(self, g, p, seed, offset, rows, cols, counter: Optional[DeviceBuffer] = None, want_dx=True,
@@ -1019,10 +1036,9 @@ class CudaBackend:
             dx = self._alloc(n)
         if dbias is None and want_dbias:
             dbias = self._alloc(cols)
-        ws, nb, hold = self._scratch(self.lib.fb_dropout_bwd_workspace_bytes(rows, cols) if dbias is not None else 0)
-        self._call(self.lib.fb_dropout_bwd, pg, rows, cols, p, seed, offset, pc,
-                                            self._want("dropout_backward: dx", dx, n),
-                                            self._want("dropout_backward: dbias", dbias, cols), ws, nb)
+        self._call_with_scratch(self.lib.fb_dropout_bwd_workspace_bytes(rows, cols) if dbias is not None else 0,
+                                self.lib.fb_dropout_bwd, pg, rows, cols, p, seed, offset, pc,
+                                self._want("dropout_backward: dx", dx, n), self._want("dropout_backward: dbias", dbias, cols))
         return dx, dbias
 
     def dropout_advance_dev(self, counter: DeviceBuffer, n):
@@ -1039,8 +1055,8 @@ class CudaBackend:
         if ids is None:
             ids = self._alloc(tokens * k, torch.int64)
         self._call(self.lib.fb_moe_gate_fwd, pl, tokens, experts, k, 1 if renorm else 0,
-                                             self._want("moe_gate: weights", weights, tokens * k),
-                                             self._want("moe_gate: ids", ids, tokens * k, i64=True))
+                   self._want("moe_gate: weights", weights, tokens * k),
+                   self._want("moe_gate: ids", ids, tokens * k, i64=True))
         return weights, ids
 
     def moe_gate_backward_dev(self, dweights, logits, weights, ids, tokens, experts, k, renorm=True, dlogits=None) -> DeviceBuffer:
@@ -1051,7 +1067,7 @@ class CudaBackend:
         if dlogits is None:
             dlogits = self._alloc(tokens * experts)
         self._call(self.lib.fb_moe_gate_bwd, pd, pl, pw, pi, tokens, experts, k, 1 if renorm else 0,
-                                             self._want("moe_gate_backward: dlogits", dlogits, tokens * experts))
+                   self._want("moe_gate_backward: dlogits", dlogits, tokens * experts))
         return dlogits
 
     def moe_sort_dev(self, ids, tokens, k, experts, place=None, order=None, offsets=None) -> MoePlan:
@@ -1065,11 +1081,9 @@ class CudaBackend:
             order = self._alloc(n, torch.int64)
         if offsets is None:
             offsets = self._alloc(experts + 1, torch.int64)
-        ws, nb, hold = self._scratch(self.lib.fb_moe_sort_workspace_bytes(n, experts))
-        self._call(self.lib.fb_moe_sort, pi, n, experts, self._want("moe_sort: place", place, n, i64=True),
-                                         self._want("moe_sort: order", order, n, i64=True),
-                                         self._want("moe_sort: offsets", offsets, experts + 1, i64=True),
-                                         self._bad_expert.data_ptr(), ws, nb)
+        self._call_with_scratch(self.lib.fb_moe_sort_workspace_bytes(n, experts), self.lib.fb_moe_sort, pi, n, experts,
+                                self._want("moe_sort: place", place, n, i64=True), self._want("moe_sort: order", order, n, i64=True),
+                                self._want("moe_sort: offsets", offsets, experts + 1, i64=True), self._bad_expert.data_ptr())
         return MoePlan(place, order, offsets, int(tokens), int(k), int(experts))
 
     def check_experts(self):
@@ -1097,7 +1111,7 @@ class CudaBackend:
             out = self._alloc(plan.tokens * plan.k * cols)
         rows = self._moe_rows("moe_dispatch", out, cols)
         self._call(self.lib.fb_moe_dispatch_fwd, px, plan.place.ptr, plan.tokens, plan.k, cols,
-                                                 self._want("moe_dispatch: out", out, rows * cols), rows)
+                   self._want("moe_dispatch: out", out, rows * cols), rows)
         return out
 
     def moe_dispatch_backward_dev(self, g, plan: MoePlan, cols, out=None) -> DeviceBuffer:
@@ -1107,7 +1121,7 @@ class CudaBackend:
         if out is None:
             out = self._alloc(plan.tokens * cols)
         self._call(self.lib.fb_moe_dispatch_bwd, pg, plan.place.ptr, plan.tokens, plan.k, cols, rows,
-                                                 self._want("moe_dispatch_backward: out", out, plan.tokens * cols))
+                   self._want("moe_dispatch_backward: out", out, plan.tokens * cols))
         return out
 
     def moe_combine_dev(self, ys, weights, plan: MoePlan, cols, out=None) -> DeviceBuffer:
@@ -1117,7 +1131,7 @@ class CudaBackend:
         if out is None:
             out = self._alloc(plan.tokens * cols)
         self._call(self.lib.fb_moe_combine_fwd, py, pw, plan.place.ptr, plan.tokens, plan.k, cols, rows,
-                                                self._want("moe_combine: out", out, plan.tokens * cols))
+                   self._want("moe_combine: out", out, plan.tokens * cols))
         return out
 
     def moe_combine_backward_dev(self, g, ys, weights, plan: MoePlan, cols, want_dys=True, want_dweights=True, dys=None,
@@ -1131,7 +1145,7 @@ class CudaBackend:
         if dweights is None and want_dweights:
             dweights = self._alloc(plan.tokens * plan.k)
         self._call(self.lib.fb_moe_combine_bwd, pg, self._want("moe_combine_backward: ys", ys, rows * cols), pw,
-                                                plan.place.ptr, plan.tokens, plan.k, cols, rows,
-                                                self._want("moe_combine_backward: dys", dys, rows * cols),
-                                                self._want("moe_combine_backward: dweights", dweights, plan.tokens * plan.k))
+                   plan.place.ptr, plan.tokens, plan.k, cols, rows,
+                   self._want("moe_combine_backward: dys", dys, rows * cols),
+                   self._want("moe_combine_backward: dweights", dweights, plan.tokens * plan.k))
         return dys, dweights

@@ -288,6 +288,7 @@ int fb_rope(fb_stream_t stream, const fb_view* x, const int64_t* positions, uint
   if (positions && position_rows != 1 && position_rows != B)
     return fail(FB_ERR_INVALID_SHAPE, "%s: %llu rows of positions for a batch of %llu", name,
                 (unsigned long long)position_rows, (unsigned long long)B);
+  if (B == 0 || S == 0 || H == 0) return FB_OK;
   fb_view o = *x;
   o.ptr = out;
   o.len = out_len;
@@ -297,7 +298,6 @@ int fb_rope(fb_stream_t stream, const fb_view* x, const int64_t* positions, uint
     o.strides[d] = out_strides ? out_strides[d] : expect;
     expect *= (int64_t)x->shape[d];
   }
-  if (B == 0 || S == 0 || H == 0) return FB_OK;
   if (int rc = check_view(name, &o)) return rc;
   if (!turns) return fail(FB_ERR_INVALID_ARG, "%s: null table of frequencies", name);
   if (B * S >= (1ull << 31) || H * D >= (1ull << 31))

@@ -523,8 +523,9 @@ FB_API int fb_mse_fwd_bwd(fb_stream_t stream, const float* pred, const float* ta
  *                  `out` is addressed by out_strides (NULL: row-major over the
  *                  shape) and out_offset in a buffer of out_len elements.  It may
  *                  be x itself (same address and strides: rotation in place,
- *                  channels from rot_dim on untouched), else the two must not
- *                  overlap, and no two elements of out may share an address.
+ *                  channels from rot_dim on untouched), else the address ranges of
+ *                  the two must be disjoint.  out's strides must nest: each steps over
+ *                  all that the smaller ones span, so no two elements share an address.
  *                  positions: device i64, row-major [position_rows, seq] with
  *                  position_rows 1 (shared) or batch; NULL: start + 0 .. seq - 1.
  *                  turns: the table in DEVICE memory.  inverse != 0 turns by

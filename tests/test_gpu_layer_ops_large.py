@@ -211,3 +211,45 @@ def test_two_backends_at_once():
             b.synchronize()
         for o, w in zip(outs, want):
             assert all(torch.equal(a.t, v) for a, v in zip(o, w))
+
+
+def test_two_threads_on_one_backend():
+    """Each call's launches share a scratch and stand together on the stream, whatever the other thread launches; a new
+    stream gets a scratch of its own."""
+    import threading
+    from ferro_b200.backend import CudaBackend
+    b = CudaBackend(0)
+    t, k, e, c = 20000, 4, 64, 96
+    data = []
+    for i in range(2):
+        r = np.random.default_rng(i)
+        data.append((b.alloc_i64_from_host(r.integers(0, e, t * k)), b.alloc_from_host(r.standard_normal((t, c)))))
+
+    def go(ids, g):
+        plan = b.moe_sort_dev(ids, t, k, e)
+        dx, db = b.dropout_backward_dev(g, 0.2, 1, 2, t, c, want_dbias=True)
+        return [plan.place.t, plan.order.t, plan.offsets.t, dx.t, db.t]
+
+    want = [go(*d) for d in data]
+    b.synchronize()
+    wrong = []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(b.stream):
+                same = [torch.stack([(a == v).all() for a, v in zip(go(*data[i]), want[i])]).all()
+                        for _ in range(100)]
+                wrong.extend(n for n, ok in enumerate(torch.stack(same).tolist()) if not ok)
+        except Exception as x:
+            wrong.append(x)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for h in threads:
+        h.start()
+    for h in threads:
+        h.join()
+    assert not wrong
+    b.stream = torch.cuda.Stream(device=b.device)
+    got = go(*data[0])
+    b.synchronize()
+    assert all(torch.equal(a, v) for a, v in zip(got, want[0]))

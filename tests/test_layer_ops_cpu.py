@@ -100,7 +100,7 @@ def test_rope_refusals(lib):
     says(lib, rope_call(lib, out=P, out_strides=(8, 16, 48, 1)), 2, "overlaps x")  # same storage, another order
     says(lib, rope_call(lib, shape=(1 << 31, 1, 1, 2), strides=(2, 2, 2, 1), rot=2, out=P + (1 << 40)), 4, "2^31")
     # nothing to do: no launch, no device
-    for shape in [(0, 3, 4, 8), (2, 0, 4, 8), (2, 3, 0, 8)]:
+    for shape in [(0, 3, 4, 8), (2, 0, 4, 8), (2, 3, 0, 8), (0, 1 << 62, 1 << 62, 8)]:
         assert rope_call(lib, shape=shape, ptr=None, out=None) == 0
 
 
@@ -220,6 +220,16 @@ def test_rope_reference_gradient_against_differences(layout):
     ang = ref.rope_angles(np.array([[5, 100, 7], [0, -3, 9]]), ref.rope_theta(6))
     got = ref.rope(up, ang, layout, 1.3, inverse=True)
     assert np.abs(got - differences(lambda z: ref.rope(z, ang, layout, 1.3), x, up)).max() < 1e-8
+
+
+def test_dropout_reference_gradient_against_differences():
+    r = np.random.default_rng(4)
+    x, b, res, up = r.standard_normal((3, 5)), r.standard_normal(5), r.standard_normal((3, 5)), r.standard_normal((3, 5))
+    p, seed, off = float(np.float32(0.4)), 9, 11
+    dx = ref.dropout(up, None, None, p, seed, off)[0]
+    assert np.abs(dx - differences(lambda z: ref.dropout(z, b, res, p, seed, off)[0], x, up)).max() < 1e-8
+    assert np.abs(dx.sum(0) - differences(lambda z: ref.dropout(x, z, res, p, seed, off)[0], b, up)).max() < 1e-8
+    assert np.abs(up - differences(lambda z: ref.dropout(x, b, z, p, seed, off)[0], res, up)).max() < 1e-8
 
 
 @pytest.mark.parametrize("renorm", [True, False])
