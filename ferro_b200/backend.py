@@ -1103,6 +1103,9 @@ class CudaBackend:
             raise InvalidShape(f"{what}: {len(buf)} elements are not rows of {cols}")
         return len(buf) // cols
 
+    def _place(self, plan):
+        return self._want("moe plan: place", plan.place, plan.tokens * plan.k, i64=True)
+
     def moe_dispatch_dev(self, x, plan: MoePlan, cols, out=None) -> DeviceBuffer:
         """xs[place[t, j]] = x[t]; rows of xs behind the last assignment are left as they were (in a buffer allocated here:
         uninitialised)."""
@@ -1110,7 +1113,7 @@ class CudaBackend:
         if out is None:
             out = self._alloc(plan.tokens * plan.k * cols)
         rows = self._moe_rows("moe_dispatch", out, cols)
-        self._call(self.lib.fb_moe_dispatch_fwd, px, plan.place.ptr, plan.tokens, plan.k, cols,
+        self._call(self.lib.fb_moe_dispatch_fwd, px, self._place(plan), plan.tokens, plan.k, cols,
                    self._want("moe_dispatch: out", out, rows * cols), rows)
         return out
 
@@ -1120,7 +1123,7 @@ class CudaBackend:
         pg = self._want("moe_dispatch_backward: g", g, rows * cols)
         if out is None:
             out = self._alloc(plan.tokens * cols)
-        self._call(self.lib.fb_moe_dispatch_bwd, pg, plan.place.ptr, plan.tokens, plan.k, cols, rows,
+        self._call(self.lib.fb_moe_dispatch_bwd, pg, self._place(plan), plan.tokens, plan.k, cols, rows,
                    self._want("moe_dispatch_backward: out", out, plan.tokens * cols))
         return out
 
@@ -1130,7 +1133,7 @@ class CudaBackend:
         py, pw = self._want("moe_combine: ys", ys, rows * cols), self._want("moe_combine: weights", weights, plan.tokens * plan.k)
         if out is None:
             out = self._alloc(plan.tokens * cols)
-        self._call(self.lib.fb_moe_combine_fwd, py, pw, plan.place.ptr, plan.tokens, plan.k, cols, rows,
+        self._call(self.lib.fb_moe_combine_fwd, py, pw, self._place(plan), plan.tokens, plan.k, cols, rows,
                    self._want("moe_combine: out", out, plan.tokens * cols))
         return out
 
@@ -1145,7 +1148,7 @@ class CudaBackend:
         if dweights is None and want_dweights:
             dweights = self._alloc(plan.tokens * plan.k)
         self._call(self.lib.fb_moe_combine_bwd, pg, self._want("moe_combine_backward: ys", ys, rows * cols), pw,
-                   plan.place.ptr, plan.tokens, plan.k, cols, rows,
+                   self._place(plan), plan.tokens, plan.k, cols, rows,
                    self._want("moe_combine_backward: dys", dys, rows * cols),
                    self._want("moe_combine_backward: dweights", dweights, plan.tokens * plan.k))
         return dys, dweights

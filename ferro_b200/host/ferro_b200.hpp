@@ -88,8 +88,11 @@ class CudaBackend {
   explicit CudaBackend(int ordinal = 0) : ordinal_(ordinal) {
     cuda_check(cudaSetDevice(ordinal), "cudaSetDevice");
     cuda_check(cudaStreamCreateWithFlags(&stream_, cudaStreamNonBlocking), "cudaStreamCreate");
+    bad_expert_ = alloc_uninit(1, DType::I64);
+    clear_bad_expert();
   }
   ~CudaBackend() {
+    bad_expert_.reset();  // on its stream
     if (scratch_) cudaFree(scratch_);
     if (stream_) cudaStreamDestroy(stream_);
   }
@@ -382,32 +385,41 @@ class CudaBackend {
     check(fb_moe_gate_bwd(s(), dweights.f32(), logits.f32(), weights.f32(), ids.i64(), tokens, experts, k, renorm ? 1 : 0, dl->f32()));
     return dl;
   }
+  // An id outside [-1, experts) counts as -1 and is reported by check_experts().
   MoePlan moe_sort_dev(const DeviceBuffer& ids, uint64_t tokens, uint64_t k, uint64_t experts) {
     const uint64_t n = tokens * k;
     want(ids, n, DType::I64);
     MoePlan p{alloc_uninit(n, DType::I64), alloc_uninit(n, DType::I64), alloc_uninit(experts + 1, DType::I64), tokens, k, experts};
     const uint64_t ws = fb_moe_sort_workspace_bytes(n, experts);
-    check(fb_moe_sort(s(), ids.i64(), n, experts, p.place->i64(), p.order->i64(), p.offsets->i64(), nullptr, scratch(ws), ws));
+    check(fb_moe_sort(s(), ids.i64(), n, experts, p.place->i64(), p.order->i64(), p.offsets->i64(), bad_expert_->i64(),
+                      scratch(ws), ws));
     return p;
+  }
+  // Throws if a moe_sort_dev since the last check saw an expert id out of range.
+  void check_experts() {
+    const int64_t bad = copy_i64_to_host(*bad_expert_)[0];
+    if (!bad) return;
+    clear_bad_expert();
+    throw InvalidShape("moe_sort: expert id at assignment " + std::to_string(bad - 1) + " out of range");
   }
   // Expert-sorted rows of tokens * k; those behind the last assignment are left uninitialised.
   Buf moe_dispatch_dev(const DeviceBuffer& x, const MoePlan& p, uint64_t cols) {
     want(x, p.tokens * cols);
     Buf xs = alloc_uninit(p.tokens * p.k * cols);
-    check(fb_moe_dispatch_fwd(s(), x.f32(), p.place->i64(), p.tokens, p.k, cols, xs->f32(), p.tokens * p.k));
+    check(fb_moe_dispatch_fwd(s(), x.f32(), place(p), p.tokens, p.k, cols, xs->f32(), p.tokens * p.k));
     return xs;
   }
   Buf moe_dispatch_backward_dev(const DeviceBuffer& g, const MoePlan& p, uint64_t cols) {
     want(g, p.tokens * p.k * cols);
     Buf dx = alloc_uninit(p.tokens * cols);
-    check(fb_moe_dispatch_bwd(s(), g.f32(), p.place->i64(), p.tokens, p.k, cols, p.tokens * p.k, dx->f32()));
+    check(fb_moe_dispatch_bwd(s(), g.f32(), place(p), p.tokens, p.k, cols, p.tokens * p.k, dx->f32()));
     return dx;
   }
   Buf moe_combine_dev(const DeviceBuffer& ys, const DeviceBuffer& weights, const MoePlan& p, uint64_t cols) {
     want(ys, p.tokens * p.k * cols);
     want(weights, p.tokens * p.k);
     Buf y = alloc_uninit(p.tokens * cols);
-    check(fb_moe_combine_fwd(s(), ys.f32(), weights.f32(), p.place->i64(), p.tokens, p.k, cols, p.tokens * p.k, y->f32()));
+    check(fb_moe_combine_fwd(s(), ys.f32(), weights.f32(), place(p), p.tokens, p.k, cols, p.tokens * p.k, y->f32()));
     return y;
   }
   // (dys, dweights)
@@ -417,7 +429,7 @@ class CudaBackend {
     want(ys, p.tokens * p.k * cols);
     want(weights, p.tokens * p.k);
     Buf dys = alloc_uninit(p.tokens * p.k * cols), dw = alloc_uninit(p.tokens * p.k);
-    check(fb_moe_combine_bwd(s(), g.f32(), ys.f32(), weights.f32(), p.place->i64(), p.tokens, p.k, cols, p.tokens * p.k, dys->f32(), dw->f32()));
+    check(fb_moe_combine_bwd(s(), g.f32(), ys.f32(), weights.f32(), place(p), p.tokens, p.k, cols, p.tokens * p.k, dys->f32(), dw->f32()));
     return {std::move(dys), std::move(dw)};
   }
 
@@ -426,6 +438,11 @@ class CudaBackend {
     if (b.dtype() != dt) throw Unsupported(dt == DType::F32 ? "an f32 buffer is needed" : "an i64 buffer is needed");
     if (b.len() != n) throw InvalidShape("buffer has " + std::to_string(b.len()) + " elements, expected " + std::to_string(n));
   }
+  static const int64_t* place(const MoePlan& p) {
+    want(*p.place, p.tokens * p.k, DType::I64);
+    return p.place->i64();
+  }
+  void clear_bad_expert() { cuda_check(cudaMemsetAsync(bad_expert_->raw(), 0, sizeof(int64_t), stream_), "cudaMemset"); }
   Buf rope(const DeviceBuffer& x, const std::vector<uint64_t>& shape, const RopePlan& plan, const DeviceBuffer* positions,
            int64_t start, int inverse) {
     if (shape.size() != 4) throw InvalidShape("rope: the shape is not [batch, seq, heads, head_dim]");
@@ -475,6 +492,7 @@ class CudaBackend {
   }
   int ordinal_;
   cudaStream_t stream_ = nullptr;
+  Buf bad_expert_;  // i64 [1], see check_experts
   void* scratch_ = nullptr;
   uint64_t scratch_bytes_ = 0;
 };

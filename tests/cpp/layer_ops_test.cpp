@@ -62,6 +62,20 @@ int main() {
     auto [dys, dww] = be.moe_combine_backward_dev(*x, *xs, *w, plan, 1);
     auto dv = be.copy_to_host(*dww);
     EXPECT(dv[0] == 1.f && dv[1] == 1.f && dv[2] == 0.f && dv[3] == 0.f && dv[4] == 9.f && dv[5] == 9.f);
+    be.check_experts();
+    auto wrong = be.alloc_i64_from_host({2, 3, 0, -2, 1, 0});
+    auto partial = be.moe_sort_dev(*wrong, 3, 2, 3);
+    auto at = be.copy_i64_to_host(*partial.place);
+    EXPECT(at[0] == 3 && at[1] == -1 && at[2] == 0 && at[3] == -1 && at[4] == 2 && at[5] == 1);
+    std::string said;
+    try { be.check_experts(); } catch (const fb::InvalidShape& e) { said = e.what(); }
+    EXPECT(said.find("assignment 3 ") != std::string::npos);
+    be.check_experts();  // said once
+    partial.tokens = 4;  // places of three tokens
+    bool refused = false;
+    auto four = be.alloc_from_host({1.f, 2.f, 3.f, 4.f});
+    try { be.moe_dispatch_dev(*four, partial, 1); } catch (const fb::InvalidShape&) { refused = true; }
+    EXPECT(refused);
   }
   std::printf("layer_ops_test ok, %llu kernel launches\n", (unsigned long long)fb_launch_count());
   return 0;

@@ -469,6 +469,21 @@ def test_rows_with_fewer_slots_than_places_and_foreign_addresses(be):
         be.moe_sort_dev(be.alloc_from_host(np.zeros(8, np.float32)), 8, 1, 4)
 
 
+def test_rows_refuse_a_plan_whose_places_do_not_fit_it(be):
+    from dataclasses import replace
+    b = bk()
+    t, e, k, c = 6, 3, 2, 8
+    plan = be.moe_sort_dev(be.alloc_i64_from_host(np.arange(t * k) % e), t, k, e)
+    x, ys, w = (be.alloc_from_host(np.ones(n, np.float32)) for n in (t * c, t * k * c, t * k))
+    calls = [lambda p: be.moe_dispatch_dev(x, p, c), lambda p: be.moe_dispatch_backward_dev(ys, p, c),
+             lambda p: be.moe_combine_dev(ys, w, p, c), lambda p: be.moe_combine_backward_dev(x, ys, w, p, c)]
+    for call in calls:
+        with pytest.raises(b.InvalidShape, match="place"):
+            call(replace(plan, place=be.alloc_i64_from_host(np.zeros(t * k - 1, np.int64))))
+        with pytest.raises(b.Unsupported, match="i64"):
+            call(replace(plan, place=w))
+
+
 # ---- the layer's run -------------------------------------------------------------------------------------------------------
 
 def test_a_layer_with_routed_experts_forward_and_backward(be):
