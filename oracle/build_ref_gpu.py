@@ -63,7 +63,7 @@ DEFAULT_ROOT = os.environ.get("FERRO_SOURCE") or os.path.join(os.sep, "root", "r
 
 
 def build(root=DEFAULT_ROOT, force=False):
-    if not os.path.isdir(root):
+    if not os.path.exists(os.path.join(root, "crates", "ferro-cuda", "src", "kernels.rs")):  # an empty folder is no source either
         return OUT if os.path.exists(OUT) else None
     if not force and os.path.exists(OUT) and os.path.getmtime(OUT) >= max(os.path.getmtime(LAUNCHER), os.path.getmtime(__file__)):
         return OUT
