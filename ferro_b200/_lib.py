@@ -228,5 +228,8 @@ def load():
         fn = getattr(lib, name)  # AttributeError if the symbol is not exported
         fn.restype = res
         fn.argtypes = args
+    # Of the CUDA runtime that the library is linked to: whether a stream is being captured, whichever stream is current.
+    lib.cudaStreamIsCapturing.restype = C.c_int
+    lib.cudaStreamIsCapturing.argtypes = [c_stream, C.POINTER(C.c_int)]
     _LIB = lib
     return lib

@@ -268,6 +268,14 @@ class CudaBackend:
     def _s(self):
         return self._stream_handle
 
+    def _capturing(self, handle=None):
+        """Whether this backend's stream (or that of `handle`) is being captured into a graph, current in torch or not."""
+        status = C.c_int()
+        rc = self.lib.cudaStreamIsCapturing(self._stream_handle if handle is None else handle, C.byref(status))
+        if rc != 0:
+            raise FerroError(f"CUDA error {rc} asking whether a stream is being captured")
+        return status.value != 0
+
     def _check(self, rc):
         if rc != 0:
             msg = self.lib.fb_last_error().decode()
@@ -937,7 +945,7 @@ class CudaBackend:
         pool, so that graphs share none with each other or with eager calls."""
         if not nbytes:
             self._call(fn, *args, None, 0)
-        elif torch.cuda.is_current_stream_capturing():
+        elif self._capturing():
             with torch.cuda.stream(self.stream):
                 t = torch.empty(int(nbytes), dtype=torch.uint8, device=self.device)
             self._call(fn, *args, t.data_ptr(), int(nbytes))
