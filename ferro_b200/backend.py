@@ -250,7 +250,7 @@ class CudaBackend:
         torch.cuda.set_device(self.device)
         # One non-default stream per backend, like lib.rs:308-312.
         self.stream = torch.cuda.Stream(device=self.device)
-        self._ws = None
+        self._ws = self._ws_of_capture = None
         self._scratch_lock = threading.Lock()  # see _call_with_scratch
         with torch.cuda.stream(self.stream):
             self._bad_expert = torch.zeros(1, dtype=torch.int64, device=self.device)  # see check_experts
@@ -291,10 +291,16 @@ class CudaBackend:
             return DeviceBuffer(torch.empty(int(n), dtype=dtype, device=self.device))
 
     def _workspace(self, nbytes):
-        """Scratch owned by the caller side of the ABI (grown on demand, reused)."""
+        """Scratch owned by the caller side of the ABI (grown on demand, reused).  During a capture it is memory of the graph's
+        pool, held until the next captured call has its own: eager scratch would be given back under the graph's launches
+        when a larger call needs more."""
         nbytes = int(nbytes)
         if nbytes == 0:
             return None, 0
+        if self._capturing():
+            with torch.cuda.stream(self.stream):
+                t = self._ws_of_capture = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)
+            return t.data_ptr(), t.numel()
         if self._ws is None or self._ws.numel() < nbytes:
             with torch.cuda.stream(self.stream):
                 self._ws = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=self.device)

@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from ferro_b200 import kinds as K
+
 pytestmark = pytest.mark.gpu
 
 
@@ -61,3 +63,31 @@ def test_a_captured_call_takes_scratch_of_the_graph_whatever_stream_is_current(b
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_a_captured_reduction_takes_scratch_of_the_graph(be):
+    """The same of the entries whose scratch comes from the shared workspace."""
+    rows, cols = 4096, 1024
+    r = np.random.default_rng(2)
+    x, g, w = (be.alloc_from_host(r.standard_normal(n)) for n in (rows * cols, rows * cols, cols))
+
+    def go():
+        y, mean, rstd = be.layer_norm_stats_dev(x, w, None, rows, cols, 1e-5)
+        dx, dw, db = be.layer_norm_backward_dev(g, w, rows, cols, x=x, mean=mean, rstd=rstd)
+        return [y.t, dx.t, dw.t, db.t, be.sum_dim_dev(g, (rows, cols), 0).t, be.reduce_dev(K.RED_SUM, x).t]
+
+    want = go()
+    be.synchronize()
+    eager = be._ws
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=be.stream):
+        outs = go()
+    assert be._ws is eager and be._ws_of_capture.data_ptr() != eager.data_ptr()
+    eager.fill_(0xFF)
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    assert bool((eager == 0xFF).all())  # the graph wrote nothing there
