@@ -248,10 +248,10 @@ class CudaBackend:
         self.lib = _lib.load()
         self.device = torch.device("cuda", ordinal)
         torch.cuda.set_device(self.device)
+        self._scratch_lock = threading.Lock()  # see _call_with_scratch
+        self._stream, self._left = None, []  # _left: streams replaced since the last check_experts
         # One non-default stream per backend, like lib.rs:308-312.
         self.stream = torch.cuda.Stream(device=self.device)
-        self._ws = self._ws_of_capture = None
-        self._scratch_lock = threading.Lock()  # see _call_with_scratch
         with torch.cuda.stream(self.stream):
             self._bad_expert = torch.zeros(1, dtype=torch.int64, device=self.device)  # see check_experts
 
@@ -262,8 +262,19 @@ class CudaBackend:
 
     @stream.setter
     def stream(self, stream):
-        self._stream, self._stream_handle = stream, C.c_void_p(stream.cuda_stream)
-        self._scratch = None  # the old stream's work may still be in it
+        """Work on the new stream follows what was given to the old one, unless one of them is being captured: a graph is
+        ordered where it is replayed.  The old stream's work may still be in its scratch: the new one gets its own."""
+        with self._scratch_lock:
+            old, handle = self._stream, C.c_void_p(stream.cuda_stream)
+            if old is not None and old == stream:
+                return
+            if old is not None:
+                if not self._capturing(self._stream_handle) and not self._capturing(handle):
+                    stream.wait_stream(old)
+                if old not in self._left:
+                    self._left.append(old)
+            self._ws = self._ws_of_capture = self._scratch = None
+            self._stream, self._stream_handle = stream, handle
 
     def _s(self):
         return self._stream_handle
@@ -1101,7 +1112,14 @@ class CudaBackend:
         return MoePlan(place, order, offsets, int(tokens), int(k), int(experts))
 
     def check_experts(self):
-        """Raises if a moe_sort_dev since the last check saw an expert id out of range."""
+        """Raises if a moe_sort_dev since the last check saw an expert id out of range, on streams that were replaced since
+        too."""
+        left, self._left = self._left, []
+        for stream in left:
+            if self._capturing(C.c_void_p(stream.cuda_stream)):
+                self._left.append(stream)
+            else:
+                stream.synchronize()
         self.synchronize()
         bad = int(self._bad_expert.item())
         if bad:

@@ -91,3 +91,94 @@ def test_a_captured_reduction_takes_scratch_of_the_graph(be):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
     assert bool((eager == 0xFF).all())  # the graph wrote nothing there
+
+
+def norm_and_sort(be, seed):
+    """A large backward whose column sums go through the workspace, a bias gradient and a sort that go through the scratch."""
+    rows, cols, e = 65536, 1024, 64
+    with torch.cuda.stream(be.stream):
+        gen = torch.Generator(device=be.device).manual_seed(seed)
+        from ferro_b200.backend import DeviceBuffer
+        x, g, w = (DeviceBuffer(torch.randn(n, device=be.device, generator=gen)) for n in (rows * cols, rows * cols, cols))
+        ids = DeviceBuffer(torch.randint(0, e, (rows,), device=be.device, generator=gen))
+
+    def go():
+        y, mean, rstd = be.layer_norm_stats_dev(x, w, None, rows, cols, 1e-5)
+        dx, dw, db = be.layer_norm_backward_dev(g, w, rows, cols, x=x, mean=mean, rstd=rstd)
+        _, bias = be.dropout_backward_dev(g, 0.3, 5, 6, rows, cols, want_dx=False, want_dbias=True)
+        plan = be.moe_sort_dev(ids, rows, 1, e)
+        return [dx.t, dw.t, db.t, bias.t, plan.place.t, plan.offsets.t]
+
+    return go
+
+
+def test_a_replaced_stream_keeps_order_and_shares_no_scratch(be):
+    """Calls on the new stream while backwards on the old one are in flight, without a wait on the host: they read what the
+    old stream wrote and disturb none of its partial sums."""
+    first, second = norm_and_sort(be, 1), norm_and_sort(be, 2)
+    want = [first(), second()]
+    be.synchronize()
+    home, away = be.stream, torch.cuda.Stream(device=be.device)
+    for _ in range(3):
+        got = [None, None]
+        for _ in range(4):
+            got[0] = first()
+        ws, scratch = be._ws.data_ptr(), be._scratch.data_ptr()
+        held = be._ws, be._scratch  # so that their addresses are not given out again
+        x = got[0][0]
+        be.stream = away
+        assert be._ws is None and be._scratch is None
+        got[1] = second()
+        from ferro_b200.backend import BinaryKind, DeviceBuffer
+        twice = be.binary_dev(BinaryKind.Add, DeviceBuffer(x), DeviceBuffer(x))  # written by the old stream
+        assert be._ws.data_ptr() != ws and be._scratch.data_ptr() != scratch
+        be.stream = home
+        again = first()
+        torch.cuda.synchronize()
+        assert torch.equal(twice.t, 2 * want[0][0])
+        for a, b in [(got[0], want[0]), (got[1], want[1]), (again, want[0])]:
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+        del held
+    be.check_experts()
+
+
+def test_a_bad_expert_seen_on_a_replaced_stream_is_reported(be):
+    busy = norm_and_sort(be, 3)
+    ids = be.alloc_i64_from_host([0, 1, 7, 1])
+    for _ in range(40):
+        busy()
+    be.moe_sort_dev(ids, 4, 1, 4)
+    be.stream = torch.cuda.Stream(device=be.device)
+    with pytest.raises(Exception, match="assignment 2 "):
+        be.check_experts()
+    be.check_experts()  # said once
+    # the first calls of a backend, on a stream set before anything else
+    from ferro_b200.backend import CudaBackend
+    b = CudaBackend(0)
+    b.stream = torch.cuda.Stream(device=b.device)
+    b.moe_sort_dev(b.alloc_i64_from_host([0, 9]), 2, 1, 4)
+    with pytest.raises(Exception, match="assignment 1 "):
+        b.check_experts()
+
+
+def test_a_stream_set_within_a_capture(be):
+    """The backend moved to a stream that is being captured, and back, with work of its own stream in flight: nothing is
+    waited for across the capture's border, the graph has scratch of its own."""
+    go = norm_and_sort(be, 4)
+    want = go()
+    be.synchronize()
+    home, graph, side = be.stream, torch.cuda.CUDAGraph(), torch.cuda.Stream(device=be.device)
+    with torch.cuda.graph(graph, stream=side):
+        be.stream = side
+        outs = go()
+        be.stream = home
+    assert be._ws is None and be._scratch is None
+    eager = go()
+    be.synchronize()
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(outs, want, eager))
+    be.check_experts()
