@@ -447,6 +447,8 @@ class CudaBackend {
            int64_t start, int inverse) {
     if (shape.size() != 4) throw InvalidShape("rope: the shape is not [batch, seq, heads, head_dim]");
     want(x, numel(shape));
+    if (!plan.turns) throw InvalidShape("rope: the plan has no table of frequencies");
+    want(*plan.turns, plan.rot_dim / 2, DType::I64);
     fb_view v = {};
     v.ptr = x.f32();
     v.len = x.len();
