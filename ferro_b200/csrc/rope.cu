@@ -2,9 +2,9 @@
 // turned by position * theta_i, forward and (with the angle negated) backward.
 //
 // Angle.  theta_i is given in turns as a 64-bit fixed-point fraction, so the
-// fraction of a turn at position p is the low 64 bits of p * turns_i: exact
-// integer arithmetic, no range reduction, the same error (|p| * 2^-65 turns) for
-// the first position and the millionth.
+// fraction of a turn at position p is the low 64 bits of p * turns_i: integer
+// arithmetic without range reduction.  The fraction's last place costs |p| * 2^-64
+// turns, the cut to 32 bits 2^-32, which is the larger up to position 2^32.
 //
 // Roofline: HBM, 8 bytes per element.  A thread owns one group of pairs of one
 // token and walks HPT heads with it, so cosine and sine are paid once per HPT

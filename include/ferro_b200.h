@@ -510,10 +510,13 @@ FB_API int fb_mse_fwd_bwd(fb_stream_t stream, const float* pred, const float* ta
  * concatenations.  Pair i of a head, (a, b), at position p becomes
  *   a' = scale * (a cos(p theta_i) - b sin(p theta_i))
  *   b' = scale * (b cos(p theta_i) + a sin(p theta_i)),    i < rot_dim / 2;
- * channels from rot_dim on are copied.  The angle is exact for any i64 position:
- * theta_i is held in turns (theta_i / 2 pi) as a 64-bit fixed-point fraction, so
- * p * theta_i modulo one turn is one wrapping integer product, off by at most
- * |p| * 2^-65 turns, where an f32 product would lose 2^-24 of the whole angle.
+ * channels from rot_dim on are copied.  theta_i is held in turns (theta_i / 2 pi)
+ * as a 64-bit fixed-point fraction, off by at most one unit of its last place
+ * where theta_i <= 1, so p * theta_i modulo one turn is one wrapping integer
+ * product; the kernel goes on with its upper 32 bits.  The angle is off by at most
+ * |p| * 2^-64 + 2^-32 turns: 2^-32 turns for all practical positions, 4e-7 radians
+ * at |p| = 2^40, nothing left at 2^63.  An f32 product would lose 2^-24 of the
+ * whole angle.
  *   fb_rope_turns  fills HOST memory with that table, rot_dim / 2 entries
  *                  (fb_rope_scaling says which theta_i; factor is used by every kind
  *                  but FB_ROPE_PLAIN, original_len / low / high by FB_ROPE_BY_PARTS);
