@@ -95,7 +95,10 @@ inline unsigned grid_full(uint64_t work_items) {
 // index arithmetic) and then blocks in pdl_wait() until that kernel has
 // completed and its writes are visible.  Rules: pdl_wait() comes before the
 // first access to global memory of any kind (a predecessor may still be
-// writing this kernel's inputs or reading its outputs); pdl_trigger() tells
+// writing this kernel's inputs or reading its outputs), except to what the
+// predecessor leaves alone, where the predecessor is known and triggers only
+// after its own pdl_wait(): all that came before it has completed then
+// (moe_place_kernel, behind the kernels that count); pdl_trigger() tells
 // the scheduler that the next kernel may start to launch once every CTA of
 // this one has passed it (or exited), so it costs this kernel nothing.  A
 // kernel that never triggers releases its dependents when it ends, and a

@@ -3,7 +3,9 @@
 
 namespace fb {
 
-// n / d for n < 2^31 with one multiply-high (d >= 1).
+// n / d for any 32-bit n and d >= 1 with one multiply-high.  With 2^shift >= d and M = 2^32 + magic =
+// (2^(32 + shift) + e) / d, 0 < e <= d, the product n M / 2^(32 + shift) exceeds n / d by
+// n e / (d 2^(32 + shift)) < 1 / d: too little to reach the next whole number.
 struct FastDiv {
   uint32_t d, magic, shift;
 };

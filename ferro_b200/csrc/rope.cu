@@ -11,8 +11,10 @@
 // heads; all of a thread's loads are issued before the first product.  Measured
 // against the copy rate: 4 x 4096 tokens of 32 heads of 128 100 % in both layouts
 // (82 us), 64 of 256 channels turned 104 %, 40 of 80 89 to 95 %, 126 channels (no
-// 16-byte access fits) 88 to 96 %, one head 62 to 82 %: bound by the instructions
-// of the angles there.
+// 16-byte access fits) 88 to 96 %, one head of 128 62 % at 65536 tokens (16.5 us),
+// 94 % at 524288 (88 us): a thread has one pair of accesses in flight and its
+// angles to form before it can store, and neither limit is reached (schedulers
+// issue in 75 % of the cycles, DRAM is busy for 68 %).
 #include <cmath>
 
 #include "common.cuh"
@@ -35,7 +37,7 @@ struct RopeArgs {
   uint32_t tpb, bpt;           // tokens per CTA; CTAs per token
   uint32_t pos_batch;          // 1: positions have a row per batch entry
   uint32_t rot, dim;
-  FastDiv d_upt, d_units, d_seq, d_bpt;
+  FastDiv d_upt, d_units, d_seq;
   uint64_t blocks;
   float scale;
   uint32_t flip;               // sign bit where the angle is negated

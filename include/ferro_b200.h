@@ -576,6 +576,7 @@ FB_API int fb_dropout_advance(fb_stream_t stream, int64_t* counter, uint64_t n);
  * (ties: lowest index first; NaN before everything, as fb_max_dim) with weights
  *   renorm != 0   softmax over the chosen k
  *   renorm == 0   the chosen entries of the softmax over all experts.
+ * An exponential e^(logit - largest) below 2^-126 counts as 0, in weights and gradients.
  * A logit of -inf is masked: never chosen.  A row with fewer than k others gets
  * id -1 and weight 0 in what is left of its k places (a padded token is a row of
  * -inf).  ids are i64 [tokens, k].  1 <= k <= min(experts, FB_MOE_MAX_K),
@@ -583,7 +584,8 @@ FB_API int fb_dropout_advance(fb_stream_t stream, int64_t* counter, uint64_t n);
  * Backward, from the saved weights and ids: dlogits [tokens, experts] in full,
  *   renorm != 0   w_j (dw_j - sum_i w_i dw_i) at ids j, 0 elsewhere (logits may be NULL)
  *   renorm == 0   p_e ([e = id j] dw_j - sum_i w_i dw_i), p recomputed from logits;
- * masked entries get 0, ids outside [0, experts) are skipped. */
+ * masked entries get 0, ids outside [0, experts) are skipped.  The others of a row are distinct, as the
+ * forward leaves them: of an id given twice one place's gradient is written, not their sum. */
 #define FB_MOE_MAX_EXPERTS 1024
 #define FB_MOE_MAX_K 32
 FB_API int fb_moe_gate_fwd(fb_stream_t stream, const float* logits, uint64_t tokens, uint64_t experts, uint64_t k,
