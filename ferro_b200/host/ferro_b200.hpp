@@ -488,7 +488,14 @@ class CudaBackend {
     if (bytes <= scratch_bytes_) return scratch_;
     synchronize();
     if (scratch_) cudaFree(scratch_);
-    cuda_check(cudaMalloc(&scratch_, bytes), "cudaMalloc(scratch)");
+    scratch_ = nullptr;  // of no size until the new one is there
+    scratch_bytes_ = 0;
+    const cudaError_t e = cudaMalloc(&scratch_, bytes);
+    if (e != cudaSuccess) {
+      scratch_ = nullptr;
+      cudaGetLastError();  // or the next launch would report it
+      cuda_check(e, "cudaMalloc(scratch)");
+    }
     scratch_bytes_ = bytes;
     return scratch_;
   }
