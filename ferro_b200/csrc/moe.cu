@@ -167,7 +167,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // kept bits with the last chosen.  Such a token is chosen again on whole keys by the whole warp.  The
 // second condition also meets a left-out entry equal to the last chosen, whose order is right already: with
 // logits rounded to bf16 32768 tokens of 128 experts, 8 choices, take 10.2 us for 7.9 (back to back in a
-// graph), with all logits equal 22.8.
+// graph, rows in L2), with all logits equal 22.8.
 //
 // Bound by the integer pipe, which issues half the rate of the others: per token of 128 experts and 8
 // choices 190 instructions, 11.6 us for 32768 tokens; one warp-wide maximum per choice took 407 (16 us).
