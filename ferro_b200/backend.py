@@ -249,7 +249,7 @@ class CudaBackend:
         self.device = torch.device("cuda", ordinal)
         torch.cuda.set_device(self.device)
         self._scratch_lock = threading.Lock()  # see _call_with_scratch
-        self._stream, self._left = None, []  # _left: streams replaced since the last check_experts
+        self._stream, self._left = None, []  # _left: ends of work on replaced streams that the present one does not wait for
         # One non-default stream per backend, like lib.rs:308-312.
         self.stream = torch.cuda.Stream(device=self.device)
         with torch.cuda.stream(self.stream):
@@ -262,17 +262,20 @@ class CudaBackend:
 
     @stream.setter
     def stream(self, stream):
-        """Work on the new stream follows what was given to the old one, unless one of them is being captured: a graph is
-        ordered where it is replayed.  The old stream's work may still be in its scratch: the new one gets its own."""
+        """Work on the new stream follows what was given to the old one, which has to exist until then, unless one of them is
+        being captured: a graph is ordered where it is replayed.  The old stream's work may still be in its scratch: the new
+        one gets its own."""
         with self._scratch_lock:
             old, handle = self._stream, C.c_void_p(stream.cuda_stream)
             if old is not None and old == stream:
                 return
             if old is not None:
-                if not self._capturing(self._stream_handle) and not self._capturing(handle):
-                    stream.wait_stream(old)
-                if old not in self._left:
-                    self._left.append(old)
+                if not self._capturing(self._stream_handle):
+                    self._left.append(old.record_event())
+                if not self._capturing(handle):
+                    for event in self._left:
+                        stream.wait_event(event)
+                    self._left = []
             self._ws = self._ws_of_capture = self._scratch = None
             self._stream, self._stream_handle = stream, handle
 
@@ -1112,14 +1115,9 @@ class CudaBackend:
         return MoePlan(place, order, offsets, int(tokens), int(k), int(experts))
 
     def check_experts(self):
-        """Raises if a moe_sort_dev since the last check saw an expert id out of range, on streams that were replaced since
-        too."""
-        left, self._left = self._left, []
-        for stream in left:
-            if self._capturing(C.c_void_p(stream.cuda_stream)):
-                self._left.append(stream)
-            else:
-                stream.synchronize()
+        """Raises if a moe_sort_dev since the last check saw an expert id out of range, on a stream replaced since then too."""
+        for event in self._left:
+            event.synchronize()
         self.synchronize()
         bad = int(self._bad_expert.item())
         if bad:

@@ -182,3 +182,28 @@ def test_a_stream_set_within_a_capture(be):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(outs, want, eager))
     be.check_experts()
+
+
+def test_a_bad_expert_seen_before_a_move_into_a_capture_is_reported(be):
+    """A captured stream waits for nothing outside its graph: what the former stream still holds is kept in mind and waited
+    for by the stream that follows."""
+    busy = norm_and_sort(be, 5)
+    ids = be.alloc_i64_from_host([0, 1, 7, 1])
+    good = be.alloc_i64_from_host([0, 1, 2, 1])
+    side, third = torch.cuda.Stream(device=be.device), torch.cuda.Stream(device=be.device)
+    busy()
+    be.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):  # the eager calls below need memory
+        for _ in range(40):
+            busy()
+        be.moe_sort_dev(ids, 4, 1, 4)  # on the backend's stream, outside the graph
+        be.stream = side
+        plan = be.moe_sort_dev(good, 4, 1, 4)
+        be.stream = third
+    with pytest.raises(Exception, match="assignment 2 "):
+        be.check_experts()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert plan.place.t.tolist() == [0, 1, 3, 2]
+    be.check_experts()
